@@ -59,6 +59,33 @@ void adam_atan2(const at::Tensor& p, const at::Tensor& g, const c10::optional<at
 void cast_f32_bf16(const at::Tensor& src, const at::Tensor& dst);
 at::Tensor device_error_word();
 bool debug_bounds_build();
+int64_t paged_max_requests();
+int64_t paged_unit_keys();
+void paged_step(const at::Tensor& tables, const at::Tensor& lengths, const at::Tensor& free_stack,
+                const at::Tensor& num_free, const at::Tensor& status, const at::Tensor& done, int64_t block_size,
+                const at::Tensor& fresh, int64_t max_new, const at::Tensor& slots, const at::Tensor& positions,
+                const at::Tensor& cu_new, const at::Tensor& kv_lengths, const at::Tensor& cu_units,
+                const at::Tensor& runs, const at::Tensor& num_runs);
+void paged_truncate(const at::Tensor& tables, const at::Tensor& lengths, const at::Tensor& free_stack,
+                    const at::Tensor& num_free, const at::Tensor& status, const at::Tensor& done, int64_t block_size,
+                    const at::Tensor& keep);
+void paged_append(const at::Tensor& key, const at::Tensor& value, const at::Tensor& keys, const at::Tensor& values,
+                  const at::Tensor& key_scales, const at::Tensor& value_scales, const at::Tensor& runs,
+                  const at::Tensor& num_runs);
+void paged_read(const at::Tensor& keys, const at::Tensor& values, const at::Tensor& key_scales,
+                const at::Tensor& value_scales, const at::Tensor& slots, const at::Tensor& out_keys,
+                const at::Tensor& out_values);
+void paged_attention(const at::Tensor& query, const at::Tensor& keys, const at::Tensor& values,
+                     const at::Tensor& key_scales, const at::Tensor& value_scales, const at::Tensor& tables,
+                     const at::Tensor& kv_lengths, const at::Tensor& cu_new, const at::Tensor& cu_units, int64_t max_new,
+                     bool causal, const c10::optional<at::Tensor>& gate, const at::Tensor& out);
+int64_t logprobs_max_top();
+void token_logprobs_fwd(const at::Tensor& logits, const at::Tensor& tokens, int64_t k, const at::Tensor& logprob,
+                        const at::Tensor& entropy, const c10::optional<at::Tensor>& stats, const at::Tensor& top_ids,
+                        const at::Tensor& top_lp);
+void token_logprobs_bwd(const at::Tensor& logits, const at::Tensor& tokens, const at::Tensor& stats,
+                        const c10::optional<at::Tensor>& g_lp, const c10::optional<at::Tensor>& g_h,
+                        const at::Tensor& grad);
 }  // namespace hrm
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -91,6 +118,16 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("ce_dlogits", &hrm::ce_dlogits);
   m.def("adam_atan2", &hrm::adam_atan2);
   m.def("cast_f32_bf16", &hrm::cast_f32_bf16);
+  m.def("paged_max_requests", &hrm::paged_max_requests);
+  m.def("paged_unit_keys", &hrm::paged_unit_keys, "keys of one unit of paged attention work");
+  m.def("paged_step", &hrm::paged_step, "assign blocks, slots and positions to the new tokens of every request");
+  m.def("paged_truncate", &hrm::paged_truncate, "cut requests to given lengths and free their surplus blocks");
+  m.def("paged_append", &hrm::paged_append, "quantise new keys / values into their blocks (8 bits, a scale a block and head)");
+  m.def("paged_read", &hrm::paged_read, "keys / values of given slots back as bf16");
+  m.def("paged_attention", &hrm::paged_attention, "attention of new tokens over the paged 8-bit cache, sigmoid gate fused");
+  m.def("logprobs_max_top", &hrm::logprobs_max_top);
+  m.def("token_logprobs_fwd", &hrm::token_logprobs_fwd, "log probabilities of tokens, entropy and top-k of logits rows");
+  m.def("token_logprobs_bwd", &hrm::token_logprobs_bwd, "gradient of token_logprobs_fwd with respect to the logits");
   m.def("device_error_word", &hrm::device_error_word);
   m.def("debug_bounds_build", &hrm::debug_bounds_build, "built with HRM_DEBUG_BOUNDS (device bounds checks)");
 }

@@ -1,0 +1,298 @@
+// The 8-bit paged KV cache: quantising new tokens into their blocks, and reading tokens back.
+//
+// One layer's cache is, for keys and for values, codes [num_blocks, H, s, 128] (int8 or e4m3)
+// and scales [num_blocks, H] fp32: a (block, head) holds s tokens whose values are code * scale,
+// so a head's tokens of one block are s * 128 consecutive bytes.
+//
+// Append. The new tokens of one block are consecutive (a "run" of paged_tables.cu). With S the
+// scale so far (0 for a block that was empty) and q the largest code (127, 448):
+//   S' = max(S, amax(new) * (1/q)),  code = round(x * (1/S')),
+// and where S' > S the block's older codes are rounded again, code' = round(code * (S * (1/S'))).
+// A block's scale only grows while it fills, so an older value is rounded again only when a
+// larger one arrives. 1/q and 1/S' are correctly rounded fp32 and every product rounds once.
+// A block that gets an infinity or a NaN gets the scale NaN and codes 0: attention over it
+// is NaN, as over the tokens themselves, but its codes stay finite, so that rows of a reused block
+// that its new owner has not written yet contribute exact zeros when they are masked.
+// Scales of non-zero tokens are at least 2^-100: 1/S' is finite, and ratios of two scales are.
+//
+// One CTA of 128 threads takes one (run, head, key or value): 16 lanes hold a row of 128 values as
+// 16-byte loads, the run stays in registers between the maximum and the rounding, so tokens are
+// read once and codes written once.
+#include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <cuda_fp8.h>
+#include <torch/types.h>
+
+#include "common.cuh"
+
+namespace hrm {
+namespace {
+
+constexpr int D = 128;
+constexpr int kThreads = 128;
+constexpr int kRowsAtOnce = kThreads / 16;
+
+template <bool FP8>
+struct Code {
+  static constexpr float kMax = FP8 ? 448.f : 127.f;
+};
+
+__device__ __forceinline__ void unpack8(const uint4& w, float (&v)[8]) {
+  const float2 a = unpack_bf16x2(w.x), b = unpack_bf16x2(w.y), c = unpack_bf16x2(w.z), d = unpack_bf16x2(w.w);
+  v[0] = a.x; v[1] = a.y; v[2] = b.x; v[3] = b.y; v[4] = c.x; v[5] = c.y; v[6] = d.x; v[7] = d.y;
+}
+
+// 8 values, already divided by the scale, to 8 codes (round to nearest even, saturating)
+template <bool FP8>
+__device__ __forceinline__ uint2 to_codes(const float (&x)[8]) {
+  uint32_t w[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    if constexpr (FP8) {
+      const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(x[4 * h], x[4 * h + 1]), __NV_SATFINITE, __NV_E4M3);
+      const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(x[4 * h + 2], x[4 * h + 3]), __NV_SATFINITE, __NV_E4M3);
+      w[h] = lo | hi << 16;
+    } else {
+      w[h] = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int c = max(-127, min(127, __float2int_rn(x[4 * h + i])));
+        w[h] |= (uint32_t)(c & 0xff) << (8 * i);
+      }
+    }
+  }
+  return make_uint2(w[0], w[1]);
+}
+
+template <bool FP8>
+__device__ __forceinline__ void from_codes(const uint2& w, float (&x)[8]) {
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const uint32_t v = h ? w.y : w.x;
+    if constexpr (FP8) {
+      const float2 a = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(v & 0xffff), __NV_E4M3)));
+      const float2 b = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(v >> 16), __NV_E4M3)));
+      x[4 * h] = a.x; x[4 * h + 1] = a.y; x[4 * h + 2] = b.x; x[4 * h + 3] = b.y;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[4 * h + i] = (float)(int8_t)(v >> (8 * i));
+    }
+  }
+}
+
+struct AppendArgs {
+  const __nv_bfloat16* x[2];  // keys, values: rows of H * 128
+  long x_st[2], x_sh[2];
+  uint8_t* codes[2];
+  float* scales[2];
+  const int4* runs;
+  const int* num_runs;
+  int H, size, T, num_blocks;
+};
+
+template <bool FP8, int ROWS>  // ROWS: rows of a run that a thread holds, size / 8
+__global__ void __launch_bounds__(kThreads) paged_append_kernel(const AppendArgs a) {
+  if ((int)blockIdx.x >= a.num_runs[0]) return;
+  const int4 run = a.runs[blockIdx.x];  // block, first offset, tokens, first row
+  const int h = blockIdx.y, which = blockIdx.z;
+  const int lane = threadIdx.x & 15, row0 = threadIdx.x >> 4;
+  // a plan of another cache or another number of rows: nothing outside the tensors is touched
+  if (run.x < 0 || run.x >= a.num_blocks || run.w < 0 || run.w + run.z > a.T || run.y + run.z > a.size) return;
+
+  const __nv_bfloat16* x = a.x[which] + run.w * a.x_st[which] + h * a.x_sh[which] + lane * 8;
+  uint4 held[ROWS];
+  uint32_t top = 0;  // bf16 magnitudes order as integers; at least 0x7f80 is not finite
+#pragma unroll
+  for (int i = 0; i < ROWS; ++i) {
+    const int r = row0 + i * kRowsAtOnce;
+    held[i] = r < run.z ? *reinterpret_cast<const uint4*>(x + r * a.x_st[which]) : make_uint4(0, 0, 0, 0);
+    const uint32_t m = __vmaxu2(__vmaxu2(held[i].x & 0x7fff7fffu, held[i].y & 0x7fff7fffu),
+                                __vmaxu2(held[i].z & 0x7fff7fffu, held[i].w & 0x7fff7fffu));
+    top = __vmaxu2(top, m);
+  }
+  top = max(top & 0xffffu, top >> 16);
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) top = max(top, __shfl_xor_sync(~0u, top, off));
+  __shared__ uint32_t s_top[kThreads / 32];
+  float* scale = a.scales[which] + (long)run.x * a.H + h;
+  const float before = run.y > 0 ? *scale : 0.f;
+  if ((threadIdx.x & 31) == 0) s_top[threadIdx.x >> 5] = top;
+  __syncthreads();  // also: every thread has read the scale
+  top = max(max(s_top[0], s_top[1]), max(s_top[2], s_top[3]));
+
+  const bool finite = top < 0x7f80u && before == before;
+  float now = __uint_as_float(top << 16) * (1.f / Code<FP8>::kMax);
+  if (top > 0) now = fmaxf(now, 0x1p-100f);
+  now = finite ? fmaxf(now, before) : __int_as_float(0x7fc00000);
+  const float inv = now > 0.f ? __frcp_rn(now) : 0.f;
+  uint8_t* codes = a.codes[which] + ((long)run.x * a.H + h) * a.size * D + lane * 8;
+  if (threadIdx.x == 0) *scale = now;
+
+  if (finite && before > 0.f && now != before) {  // the block's older tokens, to the wider range
+    const float ratio = before * inv;
+    for (int r = row0; r < run.y; r += kRowsAtOnce) {
+      uint2* p = reinterpret_cast<uint2*>(codes + r * D);
+      float v[8];
+      from_codes<FP8>(*p, v);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] *= ratio;
+      *p = to_codes<FP8>(v);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < ROWS; ++i) {
+    const int r = row0 + i * kRowsAtOnce;
+    if (r < run.z) {
+      uint2 out = make_uint2(0, 0);
+      if (finite) {
+        float v[8];
+        unpack8(held[i], v);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] *= inv;
+        out = to_codes<FP8>(v);
+      }
+      *reinterpret_cast<uint2*>(codes + (run.y + r) * D) = out;
+    }
+  }
+}
+
+// Tokens back as bf16: 16 threads a (slot, head), keys and values; slot -1 (or one outside the
+// cache) gives zeros.
+template <bool FP8>
+__global__ void __launch_bounds__(256)
+    paged_read_kernel(const uint8_t* __restrict__ kc, const uint8_t* __restrict__ vc, const float* __restrict__ ks,
+                      const float* __restrict__ vs, const int* __restrict__ slots, long items, int H, int size_log2,
+                      int num_blocks, __nv_bfloat16* __restrict__ keys, __nv_bfloat16* __restrict__ values) {
+  const int lane = threadIdx.x & 15;
+  for (long it = ((long)blockIdx.x * blockDim.x + threadIdx.x) >> 4; it < items;
+       it += ((long)gridDim.x * blockDim.x) >> 4) {
+    const long n = it / H;
+    const int h = (int)(it % H), slot = slots[n];
+    uint4 out[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
+    if (slot >= 0 && (slot >> size_log2) < num_blocks) {
+      const long bh = (long)(slot >> size_log2) * H + h;
+      const long at = ((bh << size_log2) + (slot & ((1 << size_log2) - 1))) * D + lane * 8;
+      const uint2 w[2] = {*reinterpret_cast<const uint2*>(kc + at), *reinterpret_cast<const uint2*>(vc + at)};
+      const float s[2] = {ks[bh], vs[bh]};
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        float v[8];
+        from_codes<FP8>(w[c], v);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] *= s[c];
+        out[c] = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]),
+                            pack_bf16x2(v[6], v[7]));
+      }
+    }
+    reinterpret_cast<uint4*>(keys)[it * 16 + lane] = out[0];
+    reinterpret_cast<uint4*>(values)[it * 16 + lane] = out[1];
+  }
+}
+
+// Checks one layer's cache; returns true for e4m3 codes.
+bool check_cache(const at::Tensor& keys, const at::Tensor& values, const at::Tensor& key_scales,
+                 const at::Tensor& value_scales) {
+  TORCH_CHECK(keys.is_cuda() && keys.dim() == 4 && keys.size(3) == D && keys.is_contiguous() &&
+                  (keys.scalar_type() == at::kChar || keys.scalar_type() == at::kFloat8_e4m3fn),
+              "cache: contiguous CUDA codes [blocks, heads, block size, 128], int8 or float8_e4m3fn");
+  TORCH_CHECK(values.sizes() == keys.sizes() && values.scalar_type() == keys.scalar_type() && values.is_contiguous() &&
+                  values.device() == keys.device(),
+              "cache: keys and values of one shape and type");
+  const int64_t s = keys.size(2);
+  TORCH_CHECK(s == 16 || s == 32 || s == 64 || s == 128, "block size must be 16, 32, 64 or 128");
+  for (const at::Tensor* t : {&key_scales, &value_scales})
+    TORCH_CHECK(t->dim() == 2 && t->size(0) == keys.size(0) && t->size(1) == keys.size(1) && t->is_contiguous() &&
+                    t->scalar_type() == at::kFloat && t->device() == keys.device(),
+                "cache: fp32 scales [blocks, heads]");
+  TORCH_CHECK(keys.size(0) * s < (1LL << 31), "cache: slots are int32");
+  return keys.scalar_type() == at::kFloat8_e4m3fn;
+}
+
+template <bool FP8>
+void launch_append(const AppendArgs& a, dim3 grid, cudaStream_t stream) {
+  switch (a.size) {
+    case 16: return paged_append_kernel<FP8, 2><<<grid, kThreads, 0, stream>>>(a);
+    case 32: return paged_append_kernel<FP8, 4><<<grid, kThreads, 0, stream>>>(a);
+    case 64: return paged_append_kernel<FP8, 8><<<grid, kThreads, 0, stream>>>(a);
+    default: return paged_append_kernel<FP8, 16><<<grid, kThreads, 0, stream>>>(a);
+  }
+}
+
+}  // namespace
+
+// key, value [T, H, 128] bf16 (any row and head strides of whole 16 bytes) into the blocks of the
+// step that made `runs` / `num_runs`; `max_new` bounds the tokens of a request.
+void paged_append(const at::Tensor& key, const at::Tensor& value, const at::Tensor& keys, const at::Tensor& values,
+                  const at::Tensor& key_scales, const at::Tensor& value_scales, const at::Tensor& runs,
+                  const at::Tensor& num_runs) {
+  const bool fp8 = check_cache(keys, values, key_scales, value_scales);
+  const int64_t H = keys.size(1), T = key.size(0);
+  for (const at::Tensor* t : {&key, &value})
+    TORCH_CHECK(t->device() == keys.device() && t->scalar_type() == at::kBFloat16 && t->dim() == 3 && t->size(0) == T &&
+                    t->size(1) == H && t->size(2) == D && (t->numel() == 0 || t->stride(2) == 1) &&
+                    t->stride(0) % 8 == 0 && t->stride(1) % 8 == 0 &&
+                    reinterpret_cast<uintptr_t>(t->data_ptr()) % 16 == 0,
+                "paged_append: key and value [T, heads, 128] bf16 on the cache's device, with 16-byte aligned rows");
+  TORCH_CHECK(runs.device() == keys.device() && runs.scalar_type() == at::kInt && runs.dim() == 2 && runs.size(1) == 4 &&
+                  runs.is_contiguous() && num_runs.device() == keys.device() && num_runs.scalar_type() == at::kInt &&
+                  num_runs.numel() == 1,
+              "paged_append: the step's runs");
+  TORCH_CHECK(H <= 65535, "paged_append: too many heads");
+  if (runs.size(0) == 0 || T == 0) return;
+  c10::cuda::CUDAGuard guard(keys.device());
+  AppendArgs a{};
+  const at::Tensor* x[2] = {&key, &value};
+  const at::Tensor* c[2] = {&keys, &values};
+  const at::Tensor* s[2] = {&key_scales, &value_scales};
+  for (int i = 0; i < 2; ++i) {
+    a.x[i] = reinterpret_cast<const __nv_bfloat16*>(x[i]->data_ptr());
+    a.x_st[i] = x[i]->stride(0);
+    a.x_sh[i] = x[i]->stride(1);
+    a.codes[i] = reinterpret_cast<uint8_t*>(c[i]->data_ptr());
+    a.scales[i] = s[i]->data_ptr<float>();
+  }
+  a.runs = reinterpret_cast<const int4*>(runs.data_ptr<int>());
+  a.num_runs = num_runs.data_ptr<int>();
+  a.H = (int)H;
+  a.size = (int)keys.size(2);
+  a.T = (int)T;
+  a.num_blocks = (int)keys.size(0);
+  const dim3 grid((unsigned)runs.size(0), (unsigned)H, 2);
+  cudaStream_t stream = at::cuda::getCurrentCUDAStream();
+  if (fp8)
+    launch_append<true>(a, grid, stream);
+  else
+    launch_append<false>(a, grid, stream);
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+}
+
+// slots [N] int32 -> out_keys, out_values [N, H, 128] bf16 (contiguous).
+void paged_read(const at::Tensor& keys, const at::Tensor& values, const at::Tensor& key_scales,
+                const at::Tensor& value_scales, const at::Tensor& slots, const at::Tensor& out_keys,
+                const at::Tensor& out_values) {
+  const bool fp8 = check_cache(keys, values, key_scales, value_scales);
+  const int64_t N = slots.numel(), H = keys.size(1);
+  TORCH_CHECK(slots.device() == keys.device() && slots.scalar_type() == at::kInt && slots.is_contiguous(),
+              "paged_read: contiguous int32 slots on the cache's device");
+  for (const at::Tensor* t : {&out_keys, &out_values})
+    TORCH_CHECK(t->device() == keys.device() && t->scalar_type() == at::kBFloat16 && t->is_contiguous() &&
+                    t->numel() == N * H * D,
+                "paged_read: outputs [slots, heads, 128] bf16");
+  if (N == 0) return;
+  c10::cuda::CUDAGuard guard(keys.device());
+  int size_log2 = 4;
+  while ((1 << size_log2) < keys.size(2)) ++size_log2;
+  const long items = N * H;
+  const int grid = (int)std::min<long>((items * 16 + 255) / 256, 1 << 20);
+  const auto* kc = reinterpret_cast<const uint8_t*>(keys.data_ptr());
+  const auto* vc = reinterpret_cast<const uint8_t*>(values.data_ptr());
+  auto* ok = reinterpret_cast<__nv_bfloat16*>(out_keys.data_ptr());
+  auto* ov = reinterpret_cast<__nv_bfloat16*>(out_values.data_ptr());
+  cudaStream_t stream = at::cuda::getCurrentCUDAStream();
+  auto* kernel = fp8 ? paged_read_kernel<true> : paged_read_kernel<false>;
+  kernel<<<grid, 256, 0, stream>>>(kc, vc, key_scales.data_ptr<float>(), value_scales.data_ptr<float>(),
+                                   slots.data_ptr<int>(), items, (int)H, size_log2, (int)keys.size(0), ok, ov);
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+}
+
+}  // namespace hrm

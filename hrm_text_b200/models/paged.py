@@ -1,0 +1,159 @@
+"""Plain torch forms of the paged 8-bit KV cache and the token log probabilities.
+
+The oracle of ``ops.paged`` and ``ops.logprobs``, and what the models run on the CPU: loops over
+requests and blocks, fp32 arithmetic in the kernels' order where the result is a code or an id
+(so those agree exactly). ``paged_kv_append`` and ``paged_kv_attention`` pick the kernels for CUDA caches.
+"""
+from __future__ import annotations
+
+import math
+from typing import Optional
+
+import torch
+from torch import Tensor
+
+from ..ops.paged import UNIT_KEYS, BlockTables, PagedKV8, StepPlan, paged_append, paged_attention
+
+QMAX = {torch.int8: 127.0, torch.float8_e4m3fn: 448.0}
+
+
+def step_reference(tables: BlockTables, new_tokens: Tensor, plan: StepPlan) -> None:
+    """``BlockTables.step`` on host tensors; fills ``plan`` in place."""
+    size, rows = tables.block_size, plan.slots.numel()
+    lengths, new = tables.lengths.tolist(), new_tokens.tolist()
+    blocks = lambda n: -(-n // size)  # noqa: E731
+    code, at, most = 0, -1, tables.tables.shape[1] * size
+    for i, (length, n) in enumerate(zip(lengths, new)):
+        fault = 4 if n < 0 else 5 if n > plan.max_new else 3 if length + n > most else 0
+        if fault:
+            code, at = fault, i
+            break
+    need = [max(0, blocks(length + n) - blocks(length)) for length, n in zip(lengths, new)]
+    if not code:
+        code = 2 if sum(new) > rows else 1 if sum(need) > int(tables.num_free) else 0
+    if code:
+        new, need = [0] * len(new), [0] * len(new)
+        if int(tables.status[0]) == 0:
+            tables.status.copy_(torch.tensor([code, at], dtype=torch.int32))
+    top, rank, row, units, runs = int(tables.num_free), 0, 0, 0, []
+    plan.slots.fill_(-1)
+    plan.positions.zero_()
+    for i, (length, n) in enumerate(zip(lengths, new)):
+        plan.cu_new[i], plan.cu_units[i], plan.kv_lengths[i] = row, units, length + n
+        have = blocks(length)
+        for j in range(need[i]):
+            tables.tables[i, have + j] = tables.free[top - 1 - (rank + j)]
+        rank += need[i]
+        done = 0
+        while done < n:
+            pos = length + done
+            block, off = int(tables.tables[i, pos // size]), pos % size
+            take = min(size - off, n - done)
+            runs.append((block, off, take, row + done))
+            plan.slots[row + done:row + done + take] = block * size + off + torch.arange(take, dtype=torch.int32)
+            plan.positions[row + done:row + done + take] = pos + torch.arange(take, dtype=torch.int32)
+            done += take
+        row += n
+        units += -(-(length + n) // UNIT_KEYS) if n else 0
+    plan.cu_new[-1], plan.cu_units[-1], plan.num_runs[0] = row, units, len(runs)
+    if runs:
+        plan.runs[:len(runs)] = torch.tensor(runs, dtype=torch.int32)
+    tables.lengths += torch.tensor(new, dtype=torch.int32)
+    tables.num_free -= rank
+
+
+def truncate_reference(tables: BlockTables, keep: Tensor) -> None:
+    size = tables.block_size
+    blocks = lambda n: -(-n // size)  # noqa: E731
+    kept = torch.minimum(tables.lengths, keep.clamp_min(0))
+    gone = [(i, b) for i, (k, n) in enumerate(zip(kept.tolist(), tables.lengths.tolist())) for b in range(blocks(k), blocks(n))]
+    top = int(tables.num_free)
+    for rank, (i, b) in enumerate(gone):
+        tables.free[top + len(gone) - 1 - rank] = tables.tables[i, b]
+        tables.tables[i, b] = -1
+    tables.lengths.copy_(kept)
+    tables.num_free += len(gone)
+
+
+def _codes(x: Tensor, dtype: torch.dtype) -> Tensor:
+    x = x.clamp(-QMAX[dtype], QMAX[dtype])
+    return x.round().to(dtype) if dtype == torch.int8 else x.to(dtype)
+
+
+def paged_append_reference(key: Tensor, value: Tensor, cache: PagedKV8, plan: StepPlan) -> None:
+    for block, off, take, row in plan.runs[:int(plan.num_runs)].tolist():
+        for x, codes, scales in ((key, cache.keys, cache.key_scales), (value, cache.values, cache.value_scales)):
+            x = x[row:row + take].float().transpose(0, 1)  # [heads, take, 128]
+            before = scales[block].clone() if off else torch.zeros_like(scales[block])
+            top = x.abs().amax((1, 2))
+            finite = torch.isfinite(x).all(-1).all(-1) & ~before.isnan()
+            now = top * torch.tensor(1 / QMAX[codes.dtype], dtype=torch.float32)
+            now = torch.where(top > 0, now.clamp_min(2.0 ** -100), now)
+            now = torch.where(finite, torch.maximum(now.nan_to_num(0.0), before.nan_to_num(0.0)), torch.nan)
+            inv = torch.where(now > 0, 1 / now, torch.zeros_like(now))
+            moved = finite & (before > 0) & (now != before)
+            old = codes[block, :, :off].float()
+            again = _codes(old * (before * inv).nan_to_num(0.0)[:, None, None], codes.dtype).float()
+            codes[block, :, :off] = torch.where(moved[:, None, None], again, old).to(codes.dtype)
+            fresh = torch.where(finite[:, None, None], x, torch.zeros_like(x)) * inv[:, None, None]
+            codes[block, :, off:off + take] = _codes(fresh, codes.dtype)
+            scales[block] = now
+
+
+def paged_read_reference(cache: PagedKV8, slots: Tensor) -> tuple[Tensor, Tensor]:
+    size, ids = cache.block_size, slots.long()
+    valid = (ids >= 0) & (ids < cache.keys.shape[0] * size)
+    block, off = ids.clamp(0, cache.keys.shape[0] * size - 1) // size, ids.clamp_min(0) % size
+    out = [torch.where(valid[:, None, None], c.float()[block, :, off] * s[block][..., None], 0.0).to(torch.bfloat16)
+           for c, s in ((cache.keys, cache.key_scales), (cache.values, cache.value_scales))]
+    return out[0], out[1]
+
+
+def paged_attention_reference(query: Tensor, cache: PagedKV8, plan: StepPlan, causal: bool = True,
+                              gate: Optional[Tensor] = None, dtype: torch.dtype = torch.float32) -> Tensor:
+    """``dtype`` is the arithmetic's; the result has the query's type."""
+    heads, size = cache.keys.shape[1], cache.block_size
+    group = query.shape[1] // heads
+    out = torch.zeros(query.shape, dtype=dtype, device=query.device)
+    cu = plan.cu_new.tolist()
+    for i, length in enumerate(plan.kv_lengths.tolist()):
+        n = cu[i + 1] - cu[i]
+        if n == 0:
+            continue
+        ids = plan.tables[i, :-(-length // size)].long()
+        k, v = ((c[ids].to(dtype) * s[ids].to(dtype)[..., None, None]).transpose(0, 1).reshape(heads, -1, 128)[:, :length]
+                for c, s in ((cache.keys, cache.key_scales), (cache.values, cache.value_scales)))
+        q = query[cu[i]:cu[i + 1]].to(dtype).view(n, heads, group, 128)
+        a = torch.einsum("nhgd,hkd->hngk", q, k) / math.sqrt(128)
+        if causal:
+            last = torch.arange(length - n, length, device=a.device)
+            a = a.masked_fill((torch.arange(length, device=a.device)[None] > last[:, None])[None, :, None], -math.inf)
+        out[cu[i]:cu[i + 1]] = torch.einsum("hngk,hkd->nhgd", a.softmax(-1), v).reshape(n, heads * group, 128)
+    if gate is not None:
+        out = out * torch.sigmoid(gate.to(dtype))
+    return out.to(query.dtype)
+
+
+def token_logprobs_reference(logits: Tensor, tokens: Tensor, top_k: int = 0, ignore: int = -100):
+    """``(logprobs, entropy, top_ids, top_logprobs)`` of ``logits [N, V]`` in their own type."""
+    empty = (logits == -math.inf).all(-1)
+    logp = torch.log_softmax(torch.where(empty[:, None], torch.zeros_like(logits), logits), -1)
+    logp = torch.where(empty[:, None], torch.full_like(logp, -math.inf), logp)
+    p = logp.exp()
+    entropy = -torch.where(p > 0, p * logp, torch.where(p.isnan(), p, torch.zeros_like(p))).sum(-1)
+    skip = tokens == ignore
+    wild = ~skip & ((tokens < 0) | (tokens >= logits.shape[1]))
+    lp = logp.gather(1, tokens.clamp(0, logits.shape[1] - 1)[:, None])[:, 0]
+    lp = torch.where(skip, torch.zeros_like(lp), torch.where(wild, torch.full_like(lp, math.nan), lp))
+    order = torch.sort(torch.where(logits.isnan(), torch.full_like(logits, math.inf), logits) + 0.0, dim=-1, descending=True,
+                       stable=True).indices
+    top = order[:, :top_k]
+    return lp, entropy, top, logp.gather(1, top)
+
+
+def paged_kv_append(key: Tensor, value: Tensor, cache: PagedKV8, plan: StepPlan) -> None:
+    (paged_append if cache.keys.is_cuda else paged_append_reference)(key, value, cache, plan)
+
+
+def paged_kv_attention(query: Tensor, cache: PagedKV8, plan: StepPlan, causal: bool, gate: Tensor) -> Tensor:
+    return (paged_attention if cache.keys.is_cuda else paged_attention_reference)(query, cache, plan, causal, gate)
