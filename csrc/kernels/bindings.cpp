@@ -61,28 +61,22 @@ at::Tensor device_error_word();
 bool debug_bounds_build();
 int64_t paged_max_requests();
 int64_t paged_unit_keys();
-void paged_step(const at::Tensor& tables, const at::Tensor& lengths, const at::Tensor& free_stack,
-                const at::Tensor& num_free, const at::Tensor& status, const at::Tensor& done, int64_t block_size,
-                const at::Tensor& fresh, int64_t max_new, const at::Tensor& slots, const at::Tensor& positions,
-                const at::Tensor& cu_new, const at::Tensor& kv_lengths, const at::Tensor& cu_units,
-                const at::Tensor& runs, const at::Tensor& num_runs);
+std::vector<at::Tensor> paged_step(const at::Tensor& tables, const at::Tensor& lengths, const at::Tensor& free_stack,
+                                   const at::Tensor& num_free, const at::Tensor& status, const at::Tensor& done,
+                                   int64_t block_size, const at::Tensor& fresh, int64_t rows, int64_t max_new);
 void paged_truncate(const at::Tensor& tables, const at::Tensor& lengths, const at::Tensor& free_stack,
                     const at::Tensor& num_free, const at::Tensor& status, const at::Tensor& done, int64_t block_size,
                     const at::Tensor& keep);
 void paged_append(const at::Tensor& key, const at::Tensor& value, const at::Tensor& keys, const at::Tensor& values,
                   const at::Tensor& key_scales, const at::Tensor& value_scales, const at::Tensor& runs,
-                  const at::Tensor& num_runs);
-void paged_read(const at::Tensor& keys, const at::Tensor& values, const at::Tensor& key_scales,
-                const at::Tensor& value_scales, const at::Tensor& slots, const at::Tensor& out_keys,
-                const at::Tensor& out_values);
-void paged_attention(const at::Tensor& query, const at::Tensor& keys, const at::Tensor& values,
-                     const at::Tensor& key_scales, const at::Tensor& value_scales, const at::Tensor& tables,
-                     const at::Tensor& kv_lengths, const at::Tensor& cu_new, const at::Tensor& cu_units, int64_t max_new,
-                     bool causal, const c10::optional<at::Tensor>& gate, const at::Tensor& out);
+                  const at::Tensor& meta);
+std::tuple<at::Tensor, at::Tensor> paged_read(const at::Tensor& keys, const at::Tensor& values, const at::Tensor& key_scales,
+                                              const at::Tensor& value_scales, const at::Tensor& slots);
+at::Tensor paged_attention(const at::Tensor& query, const at::Tensor& keys, const at::Tensor& values,
+                           const at::Tensor& key_scales, const at::Tensor& value_scales, const at::Tensor& tables,
+                           const at::Tensor& meta, int64_t max_new, bool causal, const c10::optional<at::Tensor>& gate);
 int64_t logprobs_max_top();
-void token_logprobs_fwd(const at::Tensor& logits, const at::Tensor& tokens, int64_t k, const at::Tensor& logprob,
-                        const at::Tensor& entropy, const c10::optional<at::Tensor>& stats, const at::Tensor& top_ids,
-                        const at::Tensor& top_lp);
+std::vector<at::Tensor> token_logprobs_fwd(const at::Tensor& logits, const at::Tensor& tokens, int64_t k, bool keep);
 void token_logprobs_bwd(const at::Tensor& logits, const at::Tensor& tokens, const at::Tensor& stats,
                         const c10::optional<at::Tensor>& g_lp, const c10::optional<at::Tensor>& g_h,
                         const at::Tensor& grad);

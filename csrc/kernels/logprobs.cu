@@ -11,10 +11,11 @@
 // vocabulary NaN.
 //
 // The k likeliest (k <= 64, larger first, the lowest index first among equals): the largest
-// value of each of 64 groups of 8 threads comes with the pass above. k groups hold a value of at
-// least the k-th largest of these 64, so that value bounds the answer from below: a second
-// look at the row (in L2) collects the few values at or above it, which are ranked by counting. Rows
-// with more of them than fit (long runs of equal values) are searched k times instead.
+// value of each of 64 groups of threads comes with the pass above. k groups hold a value of at
+// least the k-th largest of these 64, so that value bounds the answer from below. The pass has
+// noted the largest value of every 64 bytes: those that reach the bound, few more than k, are read
+// again, and their values at or above it are ranked by counting. Rows with more such values than
+// fit (long runs of equal ones) are searched k times instead.
 //
 // Gradient: dx_j = g_lp (1[j = t] - p_j) - g_H p_j (log p_j + H), one read and one write.
 #include <ATen/cuda/CUDAContext.h>
@@ -27,50 +28,69 @@
 namespace hrm {
 namespace {
 
-constexpr int kThreads = 512;
-constexpr int kGroups = 64;         // of 8 threads: the largest k
+constexpr int kGroups = 64;         // groups of threads: the largest k
 constexpr int kCandidates = 1024;   // values that are ranked by counting
+constexpr int kBatch = 4;           // 16-byte loads of a thread that are in flight together
+constexpr int kBatchBwd = 2;        // the same of the backward pass, which stores as many
+constexpr int kNoted = 8192;        // batches of a row whose largest value is kept in shared memory
 constexpr int64_t kIgnore = -100;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kGone = -1e4f;  // e^kGone is 0; keeps 0 * (x - m) finite
-
-template <typename T>
-struct Vec;
-template <>
-struct Vec<float> {
-  static constexpr int N = 4;
-};
-template <>
-struct Vec<__nv_bfloat16> {
-  static constexpr int N = 8;
-};
 
 __device__ __forceinline__ float value(float v) { return v; }
 __device__ __forceinline__ float value(__nv_bfloat16 v) { return __bfloat162float(v); }
 __device__ __forceinline__ void store(float* p, float v) { *p = v; }
 __device__ __forceinline__ void store(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
 
-__device__ __forceinline__ void load_vec(const float* p, float (&v)[4]) {
-  const float4 w = *reinterpret_cast<const float4*>(p);
-  v[0] = w.x; v[1] = w.y; v[2] = w.z; v[3] = w.w;
-}
-__device__ __forceinline__ void load_vec(const __nv_bfloat16* p, float (&v)[8]) {
-  const uint4 w = *reinterpret_cast<const uint4*>(p);
-  const float2 a = unpack_bf16x2(w.x), b = unpack_bf16x2(w.y), c = unpack_bf16x2(w.z), d = unpack_bf16x2(w.w);
-  v[0] = a.x; v[1] = a.y; v[2] = b.x; v[3] = b.y; v[4] = c.x; v[5] = c.y; v[6] = d.x; v[7] = d.y;
-}
-__device__ __forceinline__ void store_vec(float* p, const float (&v)[4]) {
-  *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
-}
-__device__ __forceinline__ void store_vec(__nv_bfloat16* p, const float (&v)[8]) {
-  *reinterpret_cast<uint4*>(p) = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]),
-                                            pack_bf16x2(v[6], v[7]));
-}
-
 __device__ __forceinline__ float max_nan(float a, float b) {
   float r;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
+}
+
+// 16 bytes of logits
+template <typename T>
+struct Vec;
+template <>
+struct Vec<float> {
+  static constexpr int N = 4;
+  static constexpr uint32_t kNothing = 0xff800000u;  // minus infinity in every place
+  static __device__ __forceinline__ void unpack(const uint4& w, float (&v)[4]) {
+    v[0] = __uint_as_float(w.x); v[1] = __uint_as_float(w.y); v[2] = __uint_as_float(w.z); v[3] = __uint_as_float(w.w);
+  }
+  static __device__ __forceinline__ uint4 pack(const float (&v)[4]) {
+    return make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+  }
+  static __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
+    return __float_as_uint(max_nan(__uint_as_float(a), __uint_as_float(b)));
+  }
+  static __device__ __forceinline__ float last_max(uint32_t a) { return __uint_as_float(a); }
+};
+template <>
+struct Vec<__nv_bfloat16> {
+  static constexpr int N = 8;
+  static constexpr uint32_t kNothing = 0xff80ff80u;
+  static __device__ __forceinline__ void unpack(const uint4& w, float (&v)[8]) {
+    const float2 a = unpack_bf16x2(w.x), b = unpack_bf16x2(w.y), c = unpack_bf16x2(w.z), d = unpack_bf16x2(w.w);
+    v[0] = a.x; v[1] = a.y; v[2] = b.x; v[3] = b.y; v[4] = c.x; v[5] = c.y; v[6] = d.x; v[7] = d.y;
+  }
+  static __device__ __forceinline__ uint4 pack(const float (&v)[8]) {
+    return make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
+  }
+  static __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+  }
+  static __device__ __forceinline__ float last_max(uint32_t a) {
+    const float2 v = unpack_bf16x2(a);
+    return max_nan(v.x, v.y);
+  }
+};
+// the largest of a vector's values, NaN if one is
+template <typename T>
+__device__ __forceinline__ uint32_t vec_max(const uint4& w) {
+  return Vec<T>::max2(Vec<T>::max2(w.x, w.y), Vec<T>::max2(w.z, w.w));
 }
 
 // A (value, index) as one number that orders larger values first and, among equals, lower
@@ -89,132 +109,202 @@ __device__ __forceinline__ float key_value(unsigned long long k) {
 
 struct Sums {
   float m, s, w;
+  // to another m, not below this one: with x - m' = (x - m) + (m - m')
+  __device__ __forceinline__ void move(float to) {
+    const float d = m == to ? 0.f : m - to, f = fast_exp2(d * kLog2e);
+    w = f * fmaf(s, fmaxf(d, kGone), w);
+    s *= f;
+    m = to;
+  }
 };
-__device__ __forceinline__ Sums join(const Sums& a, const Sums& b) {
-  const float m = fmaxf(a.m, b.m);
-  const float da = a.m == m ? 0.f : a.m - m, db = b.m == m ? 0.f : b.m - m;
-  const float fa = fast_exp2(da * kLog2e), fb = fast_exp2(db * kLog2e);
-  // W under another m: sum e^(x - m) (x - m) with x - m = (x - m_a) + (m_a - m)
-  return Sums{m, a.s * fa + b.s * fb, fa * fmaf(a.s, fmaxf(da, kGone), a.w) + fb * fmaf(b.s, fmaxf(db, kGone), b.w)};
+// the lanes' sums in every lane
+__device__ __forceinline__ Sums warp_join(Sums a) {
+  float m = a.m;
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, off));
+  a.move(m);
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) {
+    a.s += __shfl_xor_sync(~0u, a.s, off);
+    a.w += __shfl_xor_sync(~0u, a.w, off);
+  }
+  return a;
 }
 
-// Calls f(index, n values, first) for the row's elements: single ones up to a 16-byte boundary, vectors,
-// single ones at the end.
-template <typename T, typename One, typename Many>
-__device__ __forceinline__ void for_row(const T* x, int V, One one, Many many) {
-  constexpr int N = Vec<T>::N;
-  const int head = min(V, (int)((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / (int)sizeof(T));
-  const int vecs = (V - head) / N, tail = head + vecs * N;
-  if ((int)threadIdx.x < head) one((int)threadIdx.x);
-  for (int i = threadIdx.x; i < vecs; i += kThreads) many(head + i * N);
-  if (tail + (int)threadIdx.x < V) one(tail + (int)threadIdx.x);
-}
-
+// A row: single elements up to a 16-byte boundary, vectors, single ones at the end.
 template <typename T>
-__global__ void __launch_bounds__(kThreads)
+struct Row {
+  int head, vecs, tail;
+  __device__ __forceinline__ Row(const T* x, int V) {
+    head = min(V, (int)((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / (int)sizeof(T));
+    vecs = (V - head) / Vec<T>::N;
+    tail = head + vecs * Vec<T>::N;
+  }
+  // loads the thread's next vectors of the row, at vector i, i + THREADS, ...
+  template <int THREADS, int BATCH>
+  __device__ __forceinline__ void load(const T* x, int i, uint4 (&raw)[BATCH]) const {
+    const uint4* p = reinterpret_cast<const uint4*>(x + head);
+#pragma unroll
+    for (int u = 0; u < BATCH; ++u) {
+      const uint32_t z = Vec<T>::kNothing;
+      raw[u] = i + u * THREADS < vecs ? p[i + u * THREADS] : make_uint4(z, z, z, z);
+    }
+  }
+};
+
+template <typename T, int THREADS>
+__global__ void __launch_bounds__(THREADS)
     logprobs_kernel(const T* __restrict__ logits, long ld, int V, const int64_t* __restrict__ tokens, int k,
                     float* __restrict__ logprob, float* __restrict__ entropy, float* __restrict__ stats,
                     int64_t* __restrict__ top_ids, float* __restrict__ top_lp) {
-  constexpr int N = Vec<T>::N;
-  const int row = blockIdx.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const T* x = logits + row * ld;
-  Sums acc{-INFINITY, 0.f, 0.f};
-  float ref = 0.f;  // acc.m where there is one
-  float best = -INFINITY;
-  int best_j = 0x7fffffff;
-
-  const auto take = [&](const float* v, int n, int j0) {
-    float top = v[0];
-#pragma unroll
-    for (int i = 1; i < n; ++i) top = max_nan(top, v[i]);
-    if (!(top <= best) || best_j == 0x7fffffff) {  // rare after the first few
-      if (best == best) {
-#pragma unroll
-        for (int i = n - 1; i >= 0; --i)
-          if (v[i] == top || v[i] != v[i]) best_j = j0 + i;
-        best = top;
-      }
-      if (top > acc.m) {
-        const float d = acc.m - top, f = fast_exp2(d * kLog2e);
-        acc.w = f * fmaf(acc.s, fmaxf(d, kGone), acc.w);
-        acc.s *= f;
-        acc.m = ref = top;
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < n; ++i) {
-      const float d = v[i] - ref, e = fast_exp2(d * kLog2e);
-      acc.s += e;
-      acc.w = fmaf(e, fmaxf(d, kGone), acc.w);
-    }
-  };
-  for_row(
-      x, V,
-      [&](int j) {
-        const float v[1] = {value(x[j])};
-        take(v, 1, j);
-      },
-      [&](int j) {
-        float v[N];
-        load_vec(x + j, v);
-        take(v, N, j);
-      });
-
-  unsigned long long key = best_j == 0x7fffffff ? 0 : rank_key(best, best_j);
-  __shared__ Sums s_sum[kThreads / 32];
-  __shared__ unsigned long long s_group[kGroups], s_best[kGroups], s_cand[kCandidates];
+  constexpr int N = Vec<T>::N, WARPS = THREADS / 32, GROUP = THREADS / kGroups;
+  __shared__ Sums s_sum[WARPS];
+  __shared__ unsigned long long s_group[kGroups], s_cand[kCandidates];
+  __shared__ float s_m, s_log_s;
   __shared__ int s_count;
   __shared__ unsigned long long s_bound;
-#pragma unroll
-  for (int off = 16; off > 0; off >>= 1) {
-    acc = join(acc, Sums{__shfl_xor_sync(~0u, acc.m, off), __shfl_xor_sync(~0u, acc.s, off), __shfl_xor_sync(~0u, acc.w, off)});
-    if (off < 8) key = max(key, __shfl_xor_sync(~0u, key, off));
-  }
-  if (lane == 0) s_sum[warp] = acc;
-  if ((lane & 7) == 0) s_group[tid >> 3] = key;
-  if (tid == 0) s_count = 0;
-  __syncthreads();
-  acc = s_sum[0];
-#pragma unroll
-  for (int w = 1; w < kThreads / 32; ++w) acc = join(acc, s_sum[w]);
-  const float log_s = logf(acc.s);
+  extern __shared__ float s_noted[];  // [min(batches of the row, kNoted)], for k > 1
+  const int row = blockIdx.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const T* x = logits + row * ld;
+  const Row<T> r(x, V);
 
-  // the groups' values in order: thread i < 64 ranks group i
-  if (tid < kGroups) {
-    const unsigned long long mine = s_group[tid];
-    int r = 0;
-    for (int i = 0; i < kGroups; ++i) r += s_group[i] > mine || (s_group[i] == mine && i < tid);
-    if (r < kGroups) s_best[r] = mine;
-    if (r == k - 1) s_bound = mine;
+  Sums acc{-INFINITY, 0.f, 0.f};
+  float ref = 0.f;  // acc.m once a finite value was seen
+  // the largest value, NaN above all, and the first vector batch that has it: -1 for the
+  // single element before the vectors, -3 for that after them, -2 for none. Its index is looked up once the group's largest value is known.
+  float best = -INFINITY;
+  int best_i = -2;
+  const auto raise = [&](float top, int i) {
+    if (!(top <= best) || best_i == -2) {
+      if (best == best) {
+        best = top;
+        best_i = i;
+      }
+      if (top > acc.m) {
+        acc.move(top);
+        ref = top;
+      }
+    }
+  };
+  const auto add = [&](float v) {
+    const float d = v - ref, e = fast_exp2(d * kLog2e);
+    acc.s += e;
+    acc.w = fmaf(e, fmaxf(d, kGone), acc.w);
+  };
+  if (tid < r.head) {
+    const float v = value(x[tid]);
+    raise(v, -1);
+    add(v);
+  }
+  for (int i = tid; i < r.vecs; i += THREADS * kBatch) {
+    uint4 raw[kBatch];
+    r.template load<THREADS, kBatch>(x, i, raw);
+    uint32_t most = vec_max<T>(raw[0]);
+#pragma unroll
+    for (int u = 1; u < kBatch; ++u) most = Vec<T>::max2(most, vec_max<T>(raw[u]));
+    const float top = Vec<T>::last_max(most);
+    raise(top, i);
+    if (k > 1) {
+      const int b = i / (THREADS * kBatch) * THREADS + tid;
+      if (b < kNoted) s_noted[b] = top;
+    }
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+      float v[N];
+      Vec<T>::unpack(raw[u], v);
+#pragma unroll
+      for (int n = 0; n < N; ++n) add(v[n]);
+    }
+  }
+  if (r.tail + tid < V) {
+    const float v = value(x[r.tail + tid]);
+    raise(v, -3);
+    add(v);
+  }
+
+  acc = warp_join(acc);
+  if (lane == 0) s_sum[warp] = acc;
+  if (k > 0) {
+    // by value first (an index of 0 stands for all); then only the threads that hold the group's largest
+    // value look for it, in what they have just read
+    unsigned long long key = best_i == -2 ? 0 : rank_key(best, 0), most = key;
+#pragma unroll
+    for (int off = GROUP / 2; off > 0; off >>= 1) most = max(most, __shfl_xor_sync(~0u, most, off));
+    if (key != most || key == 0) {
+      key = 0;
+    } else if (best_i < 0) {
+      key = rank_key(best, best_i == -1 ? tid : r.tail + tid);
+    } else {
+      uint4 raw[kBatch];
+      r.template load<THREADS, kBatch>(x, best_i, raw);
+      int j = 0;
+#pragma unroll
+      for (int u = kBatch - 1; u >= 0; --u) {
+        float v[N];
+        Vec<T>::unpack(raw[u], v);
+#pragma unroll
+        for (int n = N - 1; n >= 0; --n)
+          if (v[n] == best || (best != best && v[n] != v[n])) j = r.head + (best_i + u * THREADS) * N + n;
+      }
+      key = rank_key(best, j);
+    }
+#pragma unroll
+    for (int off = GROUP / 2; off > 0; off >>= 1) key = max(key, __shfl_xor_sync(~0u, key, off));
+    if (tid % GROUP == 0) s_group[tid / GROUP] = key;
   }
   __syncthreads();
-  const float top = key_value(s_best[0]);
-  const bool empty = top == -INFINITY;
-  const auto logp = [&](float v) {  // of a logit of this row
-    return empty ? -INFINITY : (v - acc.m) - log_s;
-  };
-  if (tid == 0) {
-    const int64_t t = tokens[row];
-    logprob[row] = t == kIgnore ? 0.f : t < 0 || t >= V ? NAN : logp(value(x[t]));
-    const float h = empty ? 0.f : log_s - acc.w / acc.s;
-    entropy[row] = h;
-    if (stats != nullptr) {
-      stats[row * 3] = empty ? 0.f : acc.m;
-      stats[row * 3 + 1] = empty ? INFINITY : log_s;  // no probability, so no gradient
-      stats[row * 3 + 2] = h;
+  if (warp == 0) {
+    acc = warp_join(lane < WARPS ? s_sum[lane] : Sums{-INFINITY, 0.f, 0.f});
+    if (lane == 0) {
+      // nothing but minus infinities: m and S such that every logit's log p is -inf
+      const bool empty = acc.m == -INFINITY && acc.s == 0.f;
+      const float m = empty ? 0.f : acc.m, log_s = empty ? INFINITY : logf(acc.s);
+      const int64_t t = tokens[row];
+      logprob[row] = t == kIgnore ? 0.f : t < 0 || t >= V ? NAN : (value(x[t]) - m) - log_s;
+      const float h = empty ? 0.f : log_s - acc.w / acc.s;
+      entropy[row] = h;
+      if (stats != nullptr) {
+        stats[row * 3] = m;
+        stats[row * 3 + 1] = log_s;
+        stats[row * 3 + 2] = h;
+      }
+      s_m = m;
+      s_log_s = log_s;
+      s_count = 0;
     }
   }
   if (k == 0) return;
+  // the bound: the k-th largest of the groups' values
+  if (k == 1) {
+    if (warp == 1) {
+      unsigned long long most = max(s_group[lane], s_group[lane + 32]);
+#pragma unroll
+      for (int off = 16; off > 0; off >>= 1) most = max(most, __shfl_xor_sync(~0u, most, off));
+      if (lane == 0) s_bound = most;
+    }
+  } else if (tid < kGroups) {
+    const unsigned long long mine = s_group[tid];
+    int rank = 0;
+#pragma unroll 16
+    for (int i = 0; i < kGroups; ++i) {
+      const unsigned long long other = s_group[i];
+      rank += other > mine || (other == mine && i < tid);
+    }
+    if (rank == k - 1) s_bound = mine;
+  }
+  __syncthreads();
+  const float m = s_m, log_s = s_log_s;
+  const unsigned long long bound = s_bound;
   int64_t* ids = top_ids + (long)row * k;
   float* lps = top_lp + (long)row * k;
+  const auto write = [&](int at, unsigned long long key) {
+    ids[at] = key_index(key);
+    lps[at] = (key_value(key) - m) - log_s;
+  };
   if (k == 1) {
-    if (tid == 0) {
-      ids[0] = key_index(s_best[0]);
-      lps[0] = logp(top);
-    }
+    if (tid == 0) write(0, bound);
     return;
   }
-  const unsigned long long bound = s_bound;
   const auto offer = [&](float v, int j) {
     const unsigned long long c = rank_key(v, j);
     if (c >= bound) {
@@ -223,62 +313,60 @@ __global__ void __launch_bounds__(kThreads)
     }
   };
   const float bound_v = key_value(bound);
-  for_row(
-      x, V, [&](int j) { offer(value(x[j]), j); },
-      [&](int j) {
+  if (tid < r.head) offer(value(x[tid]), tid);
+  for (int i = tid; i < r.vecs; i += THREADS * kBatch) {
+    const int b = i / (THREADS * kBatch) * THREADS + tid;
+    if (b < kNoted && s_noted[b] < bound_v) continue;
+    uint4 raw[kBatch];
+    r.template load<THREADS, kBatch>(x, i, raw);
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+      if (i + u * THREADS < r.vecs && !(Vec<T>::last_max(vec_max<T>(raw[u])) < bound_v)) {
         float v[N];
-        load_vec(x + j, v);
-        float m = v[0];
+        Vec<T>::unpack(raw[u], v);
 #pragma unroll
-        for (int i = 1; i < N; ++i) m = max_nan(m, v[i]);
-        if (!(m < bound_v)) {
-#pragma unroll
-          for (int i = 0; i < N; ++i) offer(v[i], j + i);
-        }
-      });
+        for (int n = 0; n < N; ++n) offer(v[n], r.head + (i + u * THREADS) * N + n);
+      }
+    }
+  }
+  if (r.tail + tid < V) offer(value(x[r.tail + tid]), r.tail + tid);
   __syncthreads();
   const int n = s_count;
   if (n <= kCandidates) {
-    for (int c = tid; c < n; c += kThreads) {
+    for (int c = tid; c < n; c += THREADS) {
       const unsigned long long mine = s_cand[c];
-      int r = 0;
-      for (int i = 0; i < n; ++i) r += s_cand[i] > mine;
-      if (r < k) {
-        ids[r] = key_index(mine);
-        lps[r] = logp(key_value(mine));
-      }
+      int rank = 0;
+      for (int i = 0; i < n; ++i) rank += s_cand[i] > mine;
+      if (rank < k) write(rank, mine);
     }
     return;
   }
   // too many at the bound: the largest below the last one found, k times
   unsigned long long last = ~0ull;
-  for (int r = 0; r < k; ++r) {
+  for (int at = 0; at < k; ++at) {
     unsigned long long mine = 0;
-    for (int j = tid; j < V; j += kThreads) {
+    for (int j = tid; j < V; j += THREADS) {
       const unsigned long long c = rank_key(value(x[j]), j);
       if (c < last && c > mine) mine = c;
     }
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) mine = max(mine, __shfl_xor_sync(~0u, mine, off));
     __syncthreads();
-    if (lane == 0) s_best[warp] = mine;
+    if (lane == 0) s_group[warp] = mine;
     __syncthreads();
-    last = s_best[0];
-    for (int w = 1; w < kThreads / 32; ++w) last = max(last, s_best[w]);
-    if (tid == 0) {
-      ids[r] = key_index(last);
-      lps[r] = logp(key_value(last));
-    }
+    last = s_group[0];
+    for (int w = 1; w < WARPS; ++w) last = max(last, s_group[w]);
+    if (tid == 0) write(at, last);
   }
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kThreads)
+template <typename T, int THREADS>
+__global__ void __launch_bounds__(THREADS)
     logprobs_bwd_kernel(const T* __restrict__ logits, long ld, int V, const int64_t* __restrict__ tokens,
                         const float* __restrict__ stats, const float* __restrict__ g_lp,
                         const float* __restrict__ g_h, T* __restrict__ grad, long ldg) {
   constexpr int N = Vec<T>::N;
-  const int row = blockIdx.x;
+  const int row = blockIdx.x, tid = threadIdx.x;
   const T* x = logits + row * ld;
   T* out = grad + row * ldg;
   const int64_t t = tokens[row];
@@ -288,28 +376,44 @@ __global__ void __launch_bounds__(kThreads)
   if (log_s == INFINITY) glp = 0.f;  // a row of nothing
   const float gh = g_h != nullptr ? g_h[row] : 0.f;
   const float a = -(glp + gh * h);
-  // dx = p (a - g_H log p) (+ g_lp at the token)
-  const auto one = [&](float v, int j) {
+  // dx = p (a - g_H log p), and g_lp more at the token
+  const auto slope = [&](float v) {
     const float d = (v - m) - log_s;
-    const float p = fast_exp2(d * kLog2e);
-    float r = p * fmaf(-gh, fmaxf(d, kGone), a);
-    if (p == 0.f) r = 0.f;
-    return j == t ? r + glp : r;
+    return fast_exp2(d * kLog2e) * fmaf(-gh, fmaxf(d, kGone), a);
   };
+  const auto single = [&](int j) { store(out + j, slope(value(x[j])) + (j == t ? glp : 0.f)); };
   if (((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(out)) & 15) != 0) {
-    for (int j = threadIdx.x; j < V; j += kThreads) store(out + j, one(value(x[j]), j));
+    for (int j = tid; j < V; j += THREADS) single(j);
     return;
   }
-  for_row(
-      x, V, [&](int j) { store(out + j, one(value(x[j]), j)); },
-      [&](int j) {
-        float v[N];
-        load_vec(x + j, v);
+  const Row<T> r(x, V);
+  if (tid < r.head) single(tid);
+  for (int i = tid; i < r.vecs; i += THREADS * kBatchBwd) {
+    uint4 raw[kBatchBwd];
+    r.template load<THREADS, kBatchBwd>(x, i, raw);
 #pragma unroll
-        for (int i = 0; i < N; ++i) v[i] = one(v[i], j + i);
-        store_vec(out + j, v);
-      });
+    for (int u = 0; u < kBatchBwd; ++u) {
+      const int j = r.head + (i + u * THREADS) * N;
+      float v[N];
+      Vec<T>::unpack(raw[u], v);
+#pragma unroll
+      for (int n = 0; n < N; ++n) v[n] = slope(v[n]);
+      if (t >= j && t < j + N) {
+#pragma unroll
+        for (int n = 0; n < N; ++n) v[n] += j + n == t ? glp : 0.f;
+      }
+      if (i + u * THREADS < r.vecs) *reinterpret_cast<uint4*>(out + j) = Vec<T>::pack(v);
+    }
+  }
+  if (r.tail + tid < V) single(r.tail + tid);
 }
+
+// Threads for a row. Forward: few rows are served fastest by many threads each (33 rows of 32768
+// bf16: 1024 threads), many rows by small CTAs, of which an SM holds many, so that one's loads run under
+// another's reductions (8192 such rows: 128 threads 93 us, 256 97, 512 140). Backward, which reduces
+// nothing: 256 threads for rows of 64 KB and more (4096 rows of 32003 fp32: 179 us, 190 with 128),
+// 128 for shorter ones (20000 of 4096 bf16: 68 us, 88 with 256).
+bool few_rows(int64_t N) { return N <= 2 * device_sm_count(); }
 
 void check_logits(const at::Tensor& logits, const at::Tensor& tokens) {
   TORCH_CHECK(logits.is_cuda() && logits.dim() == 2 && (logits.numel() == 0 || logits.stride(1) == 1) &&
@@ -326,36 +430,37 @@ void check_logits(const at::Tensor& logits, const at::Tensor& tokens) {
 
 int64_t logprobs_max_top() { return kGroups; }
 
-// logprob, entropy [N] fp32; stats [N, 3] fp32 or none (for the gradient); top_ids int64 and
-// top_lp fp32 [N, k].
-void token_logprobs_fwd(const at::Tensor& logits, const at::Tensor& tokens, int64_t k, const at::Tensor& logprob,
-                        const at::Tensor& entropy, const c10::optional<at::Tensor>& stats, const at::Tensor& top_ids,
-                        const at::Tensor& top_lp) {
+// Returns logprob and entropy [N] fp32, top_ids int64 and top_lp fp32 [N, k], and with `keep` the
+// statistics [N, 3] fp32 that the gradient needs (else an empty tensor).
+std::vector<at::Tensor> token_logprobs_fwd(const at::Tensor& logits, const at::Tensor& tokens, int64_t k, bool keep) {
   check_logits(logits, tokens);
   const int64_t N = logits.size(0), V = logits.size(1);
   TORCH_CHECK(k >= 0 && k <= kGroups && k <= V, "token_logprobs: top_k is 0 to ", kGroups, " and at most the vocabulary");
-  for (const at::Tensor* o : {&logprob, &entropy, &top_lp})
-    TORCH_CHECK(o->device() == logits.device() && o->scalar_type() == at::kFloat && o->is_contiguous(), "token_logprobs: outputs");
-  TORCH_CHECK(logprob.numel() == N && entropy.numel() == N && top_lp.numel() == N * k && top_ids.numel() == N * k &&
-                  top_ids.scalar_type() == at::kLong && top_ids.is_contiguous() && top_ids.device() == logits.device() &&
-                  (!stats || (stats->numel() == 3 * N && stats->scalar_type() == at::kFloat && stats->is_contiguous() &&
-                              stats->device() == logits.device())),
-              "token_logprobs: outputs");
-  if (N == 0) return;
   c10::cuda::CUDAGuard guard(logits.device());
+  const auto f32 = logits.options().dtype(at::kFloat);
+  const at::Tensor logprob = at::empty({N}, f32), entropy = at::empty({N}, f32), top_lp = at::empty({N, k}, f32),
+                   top_ids = at::empty({N, k}, tokens.options()), stats = at::empty({keep ? N : 0, 3}, f32);
+  const std::vector<at::Tensor> out = {logprob, entropy, top_ids, top_lp, stats};
+  if (N == 0) return out;
   cudaStream_t stream = at::cuda::getCurrentCUDAStream();
-  float* st = stats ? stats->data_ptr<float>() : nullptr;
+  float* st = keep ? stats.data_ptr<float>() : nullptr;
   const auto run = [&](auto* x) {
     using T = std::remove_pointer_t<decltype(x)>;
-    logprobs_kernel<T><<<(unsigned)N, kThreads, 0, stream>>>(x, logits.stride(0), (int)V, tokens.data_ptr<int64_t>(), (int)k,
-                                                             logprob.data_ptr<float>(), entropy.data_ptr<float>(), st,
-                                                             top_ids.data_ptr<int64_t>(), top_lp.data_ptr<float>());
+    const bool few = few_rows(N);
+    auto* kernel = few ? logprobs_kernel<T, 1024> : logprobs_kernel<T, 128>;
+    // a batch is 64 bytes, and every thread's last one may be short
+    const int64_t batches = V * (int64_t)sizeof(T) / 64 + 2 * (few ? 1024 : 128);
+    const int noted = k > 1 ? (int)std::min<int64_t>(batches, kNoted) * 4 : 0;
+    kernel<<<(unsigned)N, few ? 1024 : 128, noted, stream>>>(x, logits.stride(0), (int)V, tokens.data_ptr<int64_t>(), (int)k,
+                                                         logprob.data_ptr<float>(), entropy.data_ptr<float>(), st,
+                                                         top_ids.data_ptr<int64_t>(), top_lp.data_ptr<float>());
   };
   if (logits.scalar_type() == at::kFloat)
     run(logits.data_ptr<float>());
   else
     run(reinterpret_cast<__nv_bfloat16*>(logits.data_ptr()));
   C10_CUDA_KERNEL_LAUNCH_CHECK();
+  return out;
 }
 
 // grad [N, V] like logits from the gradients of logprob and entropy ([N] fp32, either may be none).
@@ -381,8 +486,10 @@ void token_logprobs_bwd(const at::Tensor& logits, const at::Tensor& tokens, cons
   const float* b = g_h ? g_h->data_ptr<float>() : nullptr;
   const auto run = [&](auto* x, auto* g) {
     using T = std::remove_pointer_t<decltype(x)>;
-    logprobs_bwd_kernel<T><<<(unsigned)N, kThreads, 0, stream>>>(x, logits.stride(0), (int)V, tokens.data_ptr<int64_t>(),
-                                                                 stats.data_ptr<float>(), a, b, g, grad.stride(0));
+    const bool wide = V * (int64_t)sizeof(T) >= 64 * 1024;
+    auto* kernel = wide ? logprobs_bwd_kernel<T, 256> : logprobs_bwd_kernel<T, 128>;
+    kernel<<<(unsigned)N, wide ? 256 : 128, 0, stream>>>(x, logits.stride(0), (int)V, tokens.data_ptr<int64_t>(),
+                                                         stats.data_ptr<float>(), a, b, g, grad.stride(0));
   };
   if (logits.scalar_type() == at::kFloat)
     run(logits.data_ptr<float>(), grad.data_ptr<float>());

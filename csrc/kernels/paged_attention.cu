@@ -460,12 +460,11 @@ void launch_rows(const AttnArgs& a, int max_rows, const at::TensorOptions& opts,
 }  // namespace
 
 // query [T, Hq, 128] bf16 (row and head strides of whole 16 bytes); the cache of one layer
-// (paged_kv8.cu); tables, kv_lengths, cu_new, cu_units of the step; max_new bounds the new tokens of
-// a request; gate [T, Hq, 128] bf16 or none; out [T, Hq, 128] bf16, contiguous.
-void paged_attention(const at::Tensor& query, const at::Tensor& keys, const at::Tensor& values,
+// (paged_kv8.cu); tables and meta of the step (paged_tables.cu); max_new bounds the new tokens of a
+// request; gate [T, Hq, 128] bf16 or none. Returns [T, Hq, 128] bf16.
+at::Tensor paged_attention(const at::Tensor& query, const at::Tensor& keys, const at::Tensor& values,
                      const at::Tensor& key_scales, const at::Tensor& value_scales, const at::Tensor& tables,
-                     const at::Tensor& kv_lengths, const at::Tensor& cu_new, const at::Tensor& cu_units, int64_t max_new,
-                     bool causal, const c10::optional<at::Tensor>& gate, const at::Tensor& out) {
+                     const at::Tensor& meta, int64_t max_new, bool causal, const c10::optional<at::Tensor>& gate) {
   TORCH_CHECK(keys.is_cuda() && keys.dim() == 4 && keys.size(3) == D && keys.is_contiguous() &&
                   (keys.scalar_type() == at::kChar || keys.scalar_type() == at::kFloat8_e4m3fn) &&
                   values.sizes() == keys.sizes() && values.scalar_type() == keys.scalar_type() && values.is_contiguous() &&
@@ -486,18 +485,16 @@ void paged_attention(const at::Tensor& query, const at::Tensor& keys, const at::
               "paged_attention: query [T, heads, 128] bf16 on the cache's device, with 16-byte aligned rows and a "
               "multiple of the cache's heads");
   TORCH_CHECK(!gate || (rows_ok(*gate) && gate->sizes() == query.sizes()), "paged_attention: gate like query");
-  TORCH_CHECK(rows_ok(out) && out.sizes() == query.sizes() && out.is_contiguous(), "paged_attention: out like query, contiguous");
   TORCH_CHECK(tables.device() == keys.device() && tables.scalar_type() == at::kInt && tables.dim() == 2 &&
                   tables.stride(1) == 1,
               "paged_attention: block tables int32 [requests, blocks]");
-  for (const at::Tensor* t : {&kv_lengths, &cu_new, &cu_units})
-    TORCH_CHECK(t->device() == keys.device() && t->scalar_type() == at::kInt && t->is_contiguous(),
-                "paged_attention: the step's int32 tensors");
-  TORCH_CHECK(kv_lengths.numel() == R && cu_new.numel() == R + 1 && cu_units.numel() == R + 1,
+  TORCH_CHECK(meta.device() == keys.device() && meta.scalar_type() == at::kInt && meta.is_contiguous() &&
+                  meta.numel() == 3 * R + 3,
               "paged_attention: a step of these tables");
   TORCH_CHECK(paged_unit_keys() == kUnit, "paged_attention: unit of the step");
-  if (T == 0) return;
   c10::cuda::CUDAGuard guard(keys.device());
+  const at::Tensor out = at::empty({T, query.size(1), D}, query.options());
+  if (T == 0) return out;
   AttnArgs a{};
   a.q = reinterpret_cast<const __nv_bfloat16*>(query.data_ptr());
   a.q_st = query.stride(0);
@@ -508,9 +505,9 @@ void paged_attention(const at::Tensor& query, const at::Tensor& keys, const at::
   a.vs = value_scales.data_ptr<float>();
   a.tables = tables.data_ptr<int>();
   a.table_ld = tables.stride(0);
-  a.kv_len = kv_lengths.data_ptr<int>();
-  a.cu_new = cu_new.data_ptr<int>();
-  a.cu_units = cu_units.data_ptr<int>();
+  a.cu_new = meta.data_ptr<int>();
+  a.cu_units = a.cu_new + R + 1;
+  a.kv_len = a.cu_units + R + 1;
   a.R = (int)R;
   a.Hkv = (int)H;
   a.G = (int)(query.size(1) / H);
@@ -533,6 +530,7 @@ void paged_attention(const at::Tensor& query, const at::Tensor& keys, const at::
     launch_rows<true>(a, (int)std::max<int64_t>(max_rows, 1), query.options(), stream);
   else
     launch_rows<false>(a, (int)std::max<int64_t>(max_rows, 1), query.options(), stream);
+  return out;
 }
 
 }  // namespace hrm

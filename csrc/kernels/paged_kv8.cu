@@ -221,10 +221,10 @@ void launch_append(const AppendArgs& a, dim3 grid, cudaStream_t stream) {
 }  // namespace
 
 // key, value [T, H, 128] bf16 (any row and head strides of whole 16 bytes) into the blocks of the
-// step that made `runs` / `num_runs`; `max_new` bounds the tokens of a request.
+// step that made `runs` and `meta` (whose last element is the number of runs).
 void paged_append(const at::Tensor& key, const at::Tensor& value, const at::Tensor& keys, const at::Tensor& values,
                   const at::Tensor& key_scales, const at::Tensor& value_scales, const at::Tensor& runs,
-                  const at::Tensor& num_runs) {
+                  const at::Tensor& meta) {
   const bool fp8 = check_cache(keys, values, key_scales, value_scales);
   const int64_t H = keys.size(1), T = key.size(0);
   for (const at::Tensor* t : {&key, &value})
@@ -234,8 +234,8 @@ void paged_append(const at::Tensor& key, const at::Tensor& value, const at::Tens
                     reinterpret_cast<uintptr_t>(t->data_ptr()) % 16 == 0,
                 "paged_append: key and value [T, heads, 128] bf16 on the cache's device, with 16-byte aligned rows");
   TORCH_CHECK(runs.device() == keys.device() && runs.scalar_type() == at::kInt && runs.dim() == 2 && runs.size(1) == 4 &&
-                  runs.is_contiguous() && num_runs.device() == keys.device() && num_runs.scalar_type() == at::kInt &&
-                  num_runs.numel() == 1,
+                  runs.is_contiguous() && meta.device() == keys.device() && meta.scalar_type() == at::kInt &&
+                  meta.is_contiguous() && meta.numel() >= 6,
               "paged_append: the step's runs");
   TORCH_CHECK(H <= 65535, "paged_append: too many heads");
   if (runs.size(0) == 0 || T == 0) return;
@@ -252,7 +252,7 @@ void paged_append(const at::Tensor& key, const at::Tensor& value, const at::Tens
     a.scales[i] = s[i]->data_ptr<float>();
   }
   a.runs = reinterpret_cast<const int4*>(runs.data_ptr<int>());
-  a.num_runs = num_runs.data_ptr<int>();
+  a.num_runs = meta.data_ptr<int>() + meta.numel() - 1;
   a.H = (int)H;
   a.size = (int)keys.size(2);
   a.T = (int)T;
@@ -266,19 +266,16 @@ void paged_append(const at::Tensor& key, const at::Tensor& value, const at::Tens
   C10_CUDA_KERNEL_LAUNCH_CHECK();
 }
 
-// slots [N] int32 -> out_keys, out_values [N, H, 128] bf16 (contiguous).
-void paged_read(const at::Tensor& keys, const at::Tensor& values, const at::Tensor& key_scales,
-                const at::Tensor& value_scales, const at::Tensor& slots, const at::Tensor& out_keys,
-                const at::Tensor& out_values) {
+// slots [N] int32 -> keys, values [N, H, 128] bf16.
+std::tuple<at::Tensor, at::Tensor> paged_read(const at::Tensor& keys, const at::Tensor& values, const at::Tensor& key_scales,
+                                              const at::Tensor& value_scales, const at::Tensor& slots) {
   const bool fp8 = check_cache(keys, values, key_scales, value_scales);
   const int64_t N = slots.numel(), H = keys.size(1);
   TORCH_CHECK(slots.device() == keys.device() && slots.scalar_type() == at::kInt && slots.is_contiguous(),
               "paged_read: contiguous int32 slots on the cache's device");
-  for (const at::Tensor* t : {&out_keys, &out_values})
-    TORCH_CHECK(t->device() == keys.device() && t->scalar_type() == at::kBFloat16 && t->is_contiguous() &&
-                    t->numel() == N * H * D,
-                "paged_read: outputs [slots, heads, 128] bf16");
-  if (N == 0) return;
+  const auto opts = key_scales.options().dtype(at::kBFloat16);
+  const at::Tensor out_keys = at::empty({N, H, D}, opts), out_values = at::empty({N, H, D}, opts);
+  if (N == 0) return {out_keys, out_values};
   c10::cuda::CUDAGuard guard(keys.device());
   int size_log2 = 4;
   while ((1 << size_log2) < keys.size(2)) ++size_log2;
@@ -293,6 +290,7 @@ void paged_read(const at::Tensor& keys, const at::Tensor& values, const at::Tens
   kernel<<<grid, 256, 0, stream>>>(kc, vc, key_scales.data_ptr<float>(), value_scales.data_ptr<float>(),
                                    slots.data_ptr<int>(), items, (int)H, size_log2, (int)keys.size(0), ok, ov);
   C10_CUDA_KERNEL_LAUNCH_CHECK();
+  return {out_keys, out_values};
 }
 
 }  // namespace hrm

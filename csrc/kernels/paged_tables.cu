@@ -281,25 +281,24 @@ int log2_of(int64_t v) {
 int64_t paged_max_requests() { return kMaxRequests; }
 int64_t paged_unit_keys() { return kUnitKeys; }
 
-// One step: see the head of this file. Outputs (int32): slots, positions [rows]; cu_new,
-// cu_units [R + 1]; kv_lengths [R]; runs [max_runs, 4] (block, first offset, tokens, first row);
-// num_runs [1].
-void paged_step(const at::Tensor& tables, const at::Tensor& lengths, const at::Tensor& free_stack,
-                const at::Tensor& num_free, const at::Tensor& status, const at::Tensor& done, int64_t block_size,
-                const at::Tensor& fresh, int64_t max_new, const at::Tensor& slots, const at::Tensor& positions,
-                const at::Tensor& cu_new, const at::Tensor& kv_lengths, const at::Tensor& cu_units,
-                const at::Tensor& runs, const at::Tensor& num_runs) {
+// One step: see the head of this file. Returns int32 tensors: slots and positions [rows]; runs
+// [max_runs, 4] (block, first offset, tokens, first row); meta, which is cu_new [R + 1], cu_units
+// [R + 1], kv_lengths [R] and the number of runs, one after the other.
+std::vector<at::Tensor> paged_step(const at::Tensor& tables, const at::Tensor& lengths, const at::Tensor& free_stack,
+                                   const at::Tensor& num_free, const at::Tensor& status, const at::Tensor& done,
+                                   int64_t block_size, const at::Tensor& fresh, int64_t rows, int64_t max_new) {
   check_state(tables, lengths, free_stack, num_free, status, done, block_size);
-  const int64_t R = tables.size(0), rows = slots.numel();
-  for (const at::Tensor* t : {&fresh, &slots, &positions, &cu_new, &kv_lengths, &cu_units, &runs, &num_runs})
-    TORCH_CHECK(t->device() == tables.device() && t->scalar_type() == at::kInt && t->is_contiguous(),
-                "paged_step: contiguous int32 tensors on the tables' device");
-  TORCH_CHECK(fresh.numel() == R && positions.numel() == rows && cu_new.numel() == R + 1 && kv_lengths.numel() == R &&
-                  cu_units.numel() == R + 1 && runs.dim() == 2 && runs.size(1) == 4 && num_runs.numel() == 1,
-              "paged_step: output sizes");
-  TORCH_CHECK(runs.size(0) >= std::min(rows, rows / block_size + 2 * R), "paged_step: too few runs");
-  TORCH_CHECK(rows < (1LL << 31) - kThreads * 1024, "paged_step: too many rows");
+  const int64_t R = tables.size(0);
+  TORCH_CHECK(fresh.device() == tables.device() && fresh.scalar_type() == at::kInt && fresh.is_contiguous() &&
+                  fresh.numel() == R,
+              "paged_step: new tokens, contiguous int32 [requests] on the tables' device");
+  TORCH_CHECK(rows >= 0 && rows < (1LL << 31) - kThreads * 1024, "paged_step: number of rows");
   c10::cuda::CUDAGuard guard(tables.device());
+  const auto opts = tables.options();
+  const int64_t max_runs = std::min(rows, rows / block_size + 2 * R);
+  std::vector<at::Tensor> out = {at::empty({rows}, opts), at::empty({rows}, opts), at::empty({max_runs, 4}, opts),
+                                 at::empty({3 * R + 3}, opts)};
+  int* meta = out[3].data_ptr<int>();
   StepArgs a{};
   a.tables = tables.data_ptr<int>();
   a.table_ld = tables.stride(0);
@@ -314,20 +313,21 @@ void paged_step(const at::Tensor& tables, const at::Tensor& lengths, const at::T
   a.size_log2 = log2_of(block_size);
   a.rows = (int)rows;
   a.max_new = (int)std::min<int64_t>(max_new, INT32_MAX);
-  a.max_runs = (int)runs.size(0);
-  a.slots = slots.data_ptr<int>();
-  a.positions = positions.data_ptr<int>();
-  a.cu_new = cu_new.data_ptr<int>();
-  a.kv_lengths = kv_lengths.data_ptr<int>();
-  a.cu_units = cu_units.data_ptr<int>();
-  a.runs = reinterpret_cast<int4*>(runs.data_ptr<int>());
-  a.num_runs = num_runs.data_ptr<int>();
+  a.max_runs = (int)max_runs;
+  a.slots = out[0].data_ptr<int>();
+  a.positions = out[1].data_ptr<int>();
+  a.runs = reinterpret_cast<int4*>(out[2].data_ptr<int>());
+  a.cu_new = meta;
+  a.cu_units = meta + R + 1;
+  a.kv_lengths = meta + 2 * R + 2;
+  a.num_runs = meta + 3 * R + 2;
   const int smem = (int)(3 * R + 1) * 4;
   C10_CUDA_CHECK(ensure_dynamic_smem((const void*)paged_step_kernel, (3 * kMaxRequests + 1) * 4));
   // a CTA for each 256 rows, at most two for an SM: more would only repeat the prefix sums
   const int64_t grid = std::max<int64_t>(1, std::min<int64_t>((rows + kThreads - 1) / kThreads, 2 * device_sm_count()));
   paged_step_kernel<<<(int)grid, kThreads, smem, at::cuda::getCurrentCUDAStream()>>>(a);
   C10_CUDA_KERNEL_LAUNCH_CHECK();
+  return out;
 }
 
 void paged_truncate(const at::Tensor& tables, const at::Tensor& lengths, const at::Tensor& free_stack,

@@ -27,24 +27,14 @@ class TokenLogprobs(NamedTuple):
     top_logprobs: Optional[Tensor]
 
 
-def _forward(logits: Tensor, tokens: Tensor, top_k: int, stats: Optional[Tensor]):
-    n, dev = logits.shape[0], logits.device
-    logprobs, entropy = (torch.empty(n, dtype=torch.float32, device=dev) for _ in range(2))
-    top_ids = torch.empty((n, top_k), dtype=torch.int64, device=dev)
-    top_logprobs = torch.empty((n, top_k), dtype=torch.float32, device=dev)
-    cuda().token_logprobs_fwd(logits, tokens, top_k, logprobs, entropy, stats, top_ids, top_logprobs)
-    return logprobs, entropy, top_ids, top_logprobs
-
-
 class _TokenLogprobs(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits: Tensor, tokens: Tensor, top_k: int):
-        stats = torch.empty((logits.shape[0], 3), dtype=torch.float32, device=logits.device)
-        out = _forward(logits, tokens, top_k, stats)
+        *out, stats = cuda().token_logprobs_fwd(logits, tokens, top_k, True)
         ctx.save_for_backward(logits, tokens, stats)
         ctx.set_materialize_grads(False)
         ctx.mark_non_differentiable(out[2], out[3])
-        return out
+        return tuple(out)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
@@ -74,11 +64,12 @@ def token_logprobs(logits: Tensor, tokens: Tensor, top_k: int = 0) -> TokenLogpr
         raise ValueError(f"top_k must be 0 to {MAX_TOP_K} and at most the vocabulary, got {top_k}")
     lead = logits.shape[:-1]
     rows = logits if logits.dim() == 2 else logits.reshape(-1, logits.shape[-1])
-    ids = tokens.reshape(-1).to(torch.int64).contiguous()
+    ids = tokens if tokens.dim() == 1 and tokens.dtype == torch.int64 else tokens.reshape(-1).to(torch.int64)
+    ids = ids.contiguous()
     if torch.is_grad_enabled() and logits.requires_grad:
         out = _TokenLogprobs.apply(rows, ids, top_k)
     else:
-        out = _forward(rows, ids, top_k, None)
+        out = cuda().token_logprobs_fwd(rows, ids, top_k, False)
     if logits.dim() != 2:
         out = [out[0].view(lead), out[1].view(lead), out[2].view(*lead, top_k), out[3].view(*lead, top_k)]
     return TokenLogprobs(out[0], out[1], *((out[2], out[3]) if top_k else (None, None)))

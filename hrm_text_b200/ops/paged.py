@@ -20,7 +20,6 @@ The reference keeps one bf16 cache of the full context length for each slot
 """
 from __future__ import annotations
 
-from dataclasses import dataclass
 from typing import NamedTuple, Optional
 
 import torch
@@ -69,8 +68,7 @@ class PagedKV8(NamedTuple):
         return self.keys.shape[2]
 
 
-@dataclass(frozen=True)
-class StepPlan:
+class StepPlan(NamedTuple):
     """What one step's layers need; all tensors int32 on the tables' device.
 
     ``slots`` / ``positions`` ``[num_tokens]``: cache slot and position of each packed new token, requests
@@ -82,13 +80,27 @@ class StepPlan:
     tables: Tensor
     slots: Tensor
     positions: Tensor
-    cu_new: Tensor
-    kv_lengths: Tensor
-    cu_units: Tensor
     runs: Tensor
-    num_runs: Tensor
+    meta: Tensor  # cu_new, cu_units, kv_lengths, num_runs
     block_size: int
     max_new: int
+
+    @property
+    def cu_new(self) -> Tensor:
+        return self.meta[:self.tables.shape[0] + 1]
+
+    @property
+    def cu_units(self) -> Tensor:
+        R = self.tables.shape[0]
+        return self.meta[R + 1:2 * R + 2]
+
+    @property
+    def kv_lengths(self) -> Tensor:
+        return self.meta[2 * self.tables.shape[0] + 2:-1]
+
+    @property
+    def num_runs(self) -> Tensor:
+        return self.meta[-1:]
 
 
 class BlockTables:
@@ -138,19 +150,16 @@ class BlockTables:
         if num_tokens < 0:
             raise ValueError("num_tokens must not be negative")
         max_new = num_tokens if max_new is None else min(int(max_new), num_tokens)
-        i32 = dict(dtype=torch.int32, device=dev)
-        max_runs = min(num_tokens, num_tokens // self.block_size + 2 * R)
-        plan = StepPlan(tables=self.tables, slots=torch.empty(num_tokens, **i32), positions=torch.empty(num_tokens, **i32),
-                        cu_new=torch.empty(R + 1, **i32), kv_lengths=torch.empty(R, **i32),
-                        cu_units=torch.empty(R + 1, **i32), runs=torch.empty((max_runs, 4), **i32),
-                        num_runs=torch.empty(1, **i32), block_size=self.block_size, max_new=max_new)
         new_tokens = new_tokens.contiguous()
         if dev.type == "cuda":
-            cuda().paged_step(*self._state(), new_tokens, max_new, plan.slots, plan.positions, plan.cu_new, plan.kv_lengths,
-                              plan.cu_units, plan.runs, plan.num_runs)
-        else:
-            from ..models.paged import step_reference
-            step_reference(self, new_tokens, plan)
+            return StepPlan(self.tables, *cuda().paged_step(*self._state(), new_tokens, num_tokens, max_new),
+                            self.block_size, max_new)
+        from ..models.paged import step_reference
+        i32 = dict(dtype=torch.int32, device=dev)
+        plan = StepPlan(self.tables, torch.empty(num_tokens, **i32), torch.empty(num_tokens, **i32),
+                        torch.empty((min(num_tokens, num_tokens // self.block_size + 2 * R), 4), **i32),
+                        torch.empty(3 * R + 3, **i32), self.block_size, max_new)
+        step_reference(self, new_tokens, plan)
         return plan
 
     def truncate(self, keep: Tensor) -> None:
@@ -190,7 +199,7 @@ def paged_append(key: Tensor, value: Tensor, cache: PagedKV8, plan: StepPlan) ->
     rounded again. An infinity or NaN makes its block and head read as NaN.
     """
     _check_plan(cache, plan, key.shape[0])
-    cuda().paged_append(key, value, cache.keys, cache.values, cache.key_scales, cache.value_scales, plan.runs, plan.num_runs)
+    cuda().paged_append(key, value, cache.keys, cache.values, cache.key_scales, cache.value_scales, plan.runs, plan.meta)
 
 
 def paged_read(cache: PagedKV8, slots: Tensor) -> tuple[Tensor, Tensor]:
@@ -199,10 +208,7 @@ def paged_read(cache: PagedKV8, slots: Tensor) -> tuple[Tensor, Tensor]:
         raise RuntimeError("hrm_text_b200.ops.paged takes CUDA caches only (models.paged has the CPU oracle)")
     if slots.dtype != torch.int32 or slots.dim() != 1:
         raise ValueError("slots must be int32 [N]")
-    shape = (slots.numel(), cache.keys.shape[1], cache.keys.shape[3])
-    keys, values = (torch.empty(shape, dtype=torch.bfloat16, device=cache.keys.device) for _ in range(2))
-    cuda().paged_read(*cache, slots.contiguous(), keys, values)
-    return keys, values
+    return cuda().paged_read(*cache, slots.contiguous())
 
 
 def paged_attention(query: Tensor, cache: PagedKV8, plan: StepPlan, causal: bool = True,
@@ -215,7 +221,4 @@ def paged_attention(query: Tensor, cache: PagedKV8, plan: StepPlan, causal: bool
     zero. Returns ``[num_tokens, q_heads, 128]`` bf16.
     """
     _check_plan(cache, plan, query.shape[0])
-    out = torch.empty(query.shape, dtype=query.dtype, device=query.device)
-    cuda().paged_attention(query, *cache, plan.tables, plan.kv_lengths, plan.cu_new, plan.cu_units, plan.max_new, causal,
-                           gate, out)
-    return out
+    return cuda().paged_attention(query, *cache, plan.tables, plan.meta, plan.max_new, causal, gate)
