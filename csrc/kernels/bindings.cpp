@@ -60,7 +60,6 @@ void cast_f32_bf16(const at::Tensor& src, const at::Tensor& dst);
 at::Tensor device_error_word();
 bool debug_bounds_build();
 int64_t paged_max_requests();
-int64_t paged_unit_keys();
 std::vector<at::Tensor> paged_step(const at::Tensor& tables, const at::Tensor& lengths, const at::Tensor& free_stack,
                                    const at::Tensor& num_free, const at::Tensor& status, const at::Tensor& done,
                                    int64_t block_size, const at::Tensor& fresh, int64_t rows, int64_t max_new);
@@ -113,7 +112,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("adam_atan2", &hrm::adam_atan2);
   m.def("cast_f32_bf16", &hrm::cast_f32_bf16);
   m.def("paged_max_requests", &hrm::paged_max_requests);
-  m.def("paged_unit_keys", &hrm::paged_unit_keys, "keys of one unit of paged attention work");
   m.def("paged_step", &hrm::paged_step, "assign blocks, slots and positions to the new tokens of every request");
   m.def("paged_truncate", &hrm::paged_truncate, "cut requests to given lengths and free their surplus blocks");
   m.def("paged_append", &hrm::paged_append, "quantise new keys / values into their blocks (8 bits, a scale a block and head)");

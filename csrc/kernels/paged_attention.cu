@@ -7,22 +7,25 @@
 //   y = sigmoid(gate) * o   (when a gate is given).
 //
 // Work split. A unit is 128 keys of one (request, kv head); the units of all pairs, laid end to
-// end, are cut into equal ranges, one for each CTA (the prefix sums come with the step, see
-// paged_tables.cu). A long sequence is thus spread over many CTAs and short ones share a CTA,
-// whatever the mix of lengths. A pair inside one CTA is finished there; the parts of a pair
-// that spans CTAs go to a workspace and a second kernel joins them in order (no atomics: the
-// same inputs give the same bits).
+// end with a fixed cost before each pair, are cut into equal ranges, one for each CTA (the prefix
+// sums come with the step, see paged_tables.cu). A long sequence is thus spread over many CTAs
+// and short ones share a CTA, whatever the mix of lengths. A pair inside one CTA is finished
+// there; the parts of a pair that spans CTAs go to a workspace and a second kernel joins them in
+// order (no atomics: the same inputs give the same bits).
 //
 // In a CTA each of 8 warps takes 16 keys of a unit and keeps its own running maximum, sum and
 // output for up to 8 * NT query rows (G query heads times the request's new tokens); the
-// warps are merged through shared memory once per pair. A warp's 16 keys are
+// warps are merged through shared memory once per pair. Each warp copies its own codes ahead into
+// its own ring of shared memory (cp.async, 4 KB a stage), across the ends of pairs, so that it
+// waits for no other warp and a pair's first loads run under the work before it.
+// A warp's 16 keys are
 //   S^T [16 keys x 8 rows] = C [16 x 128] Q^T,   O^T [128 dims x 8 rows] += C'^T [128 x 16] P^T
 // in mma.m16n8k16 with the keys as the M side: 8 rows, the smallest N, waste the least of a
 // matrix instruction on the one or few rows a decode step has. The kernel is bound by reading the
 // codes (256 bytes a key and head for 4 * 128 * rows flops), so warp-level matrix instructions
-// on codes converted in registers are far from their limit and need no staging:
+// on codes converted in registers are far from their limit:
 //   * the k index of S = C Q^T may be permuted as one likes if Q is permuted alike, so a lane
-//     owns 32 dims of two keys as four 16-byte loads, and a 32-bit word of codes is the lane's
+//     owns 32 dims of two keys as four 16-byte words, and a 32-bit word of codes is the lane's
 //     part of one k step;
 //   * the m index of O^T likewise: a lane owns 16 dims of four keys, pairs of keys are
 //     interleaved by byte permutes before they are widened;
@@ -40,15 +43,15 @@
 
 #include "common.cuh"
 #include "device_setup.h"
+#include "paged.h"
 
 namespace hrm {
-int64_t paged_unit_keys();
 namespace {
 
 constexpr int D = 128;
 constexpr int kWarps = 8;
 constexpr int kThreads = kWarps * 32;
-constexpr int kUnit = 128;          // keys of a unit: 16 for each warp
+constexpr int kStage = 2 * 16 * D;  // bytes of a warp's 16 keys: codes of keys, then of values
 constexpr float kLazy = 8.f;        // a running maximum may lag by 2^8: P stays below 256 in f16
 constexpr float kMinUnit = 0x1p-64f;  // a unit is at least this part of the one before it
 
@@ -73,12 +76,9 @@ struct AttnArgs {
   float* part;  // [2 * workers][tiles][8 * NT][130]: output, maximum, sum
 };
 
-struct Place {  // a position in the units laid end to end
-  int i, h, u, nu;
-};
-
-// The (request, head, unit) at `x`; every thread of the CTA calls it.
-__device__ __forceinline__ Place find_place(const AttnArgs& a, long x) {
+// The request whose part of the costs laid end to end holds position `x`; every thread of the CTA
+// calls it.
+__device__ __forceinline__ int find_request(const AttnArgs& a, long x) {
   int i = 0;
   for (int base = 0; base < a.R; base += kThreads) {
     const int j = base + (int)threadIdx.x;
@@ -86,9 +86,64 @@ __device__ __forceinline__ Place find_place(const AttnArgs& a, long x) {
     i += c;
     if (c < kThreads) break;
   }
-  const int c0 = a.cu_units[i], nu = a.cu_units[i + 1] - c0;
-  const long in = x - (long)c0 * a.Hkv;
-  return Place{i, (int)(in / nu), (int)(in % nu), nu};
+  return i;
+}
+
+// A CTA's range of positions, walked pair by pair.
+struct Walk {
+  long x, x_end;
+  int i, c0, c1;      // a request, its first position / Hkv and its end's
+  int h, u0, u1, nu;  // units [u0, u1) of nu of a pair (i, h)
+  int row_t, n, len;  // the request's first packed row, new tokens, tokens
+
+  __device__ __forceinline__ void start(const AttnArgs& a, long from, long to, int request) {
+    x = from;
+    x_end = to;
+    i = request;
+    enter(a);
+  }
+  __device__ __forceinline__ void enter(const AttnArgs& a) {
+    c0 = a.cu_units[i];
+    c1 = a.cu_units[i + 1];
+    row_t = a.cu_new[i];
+    n = a.cu_new[i + 1] - row_t;
+    len = a.kv_len[i];
+  }
+  // The next piece of a pair with rows in tile `first_row`; false at the end.
+  __device__ __forceinline__ bool next(const AttnArgs& a, int first_row) {
+    while (x < x_end) {
+      while (x >= (long)c1 * a.Hkv) {
+        ++i;
+        enter(a);
+      }
+      const int cost = c1 - c0;
+      const long in = x - (long)c0 * a.Hkv;
+      h = (int)(in / cost);
+      const int p0 = (int)(in - (long)h * cost), p1 = (int)min((long)cost, p0 + (x_end - x));
+      x += p1 - p0;
+      u0 = max(0, p0 - kPairCost);
+      u1 = max(0, p1 - kPairCost);
+      nu = cost - kPairCost;
+      if (u1 > u0 && n * a.G > first_row) return true;
+    }
+    return false;
+  }
+  // keys that a row of the tile can see at most
+  __device__ __forceinline__ int most(const AttnArgs& a, int first_row, int rows) const {
+    return a.causal ? len - n + (first_row + rows - 1) / a.G + 1 : len;
+  }
+};
+
+__device__ __forceinline__ void copy16(void* smem, const void* global) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(smem)), "l"(global) : "memory");
+}
+__device__ __forceinline__ void copy4(void* smem, const void* global) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(smem)), "l"(global) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
 template <bool FP8>
@@ -136,13 +191,6 @@ __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
   const __half2 v = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&v);
 }
-__device__ __forceinline__ uint4 load_codes(const uint8_t* p) {  // read once: leave L1 to others
-  uint4 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
-               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-               : "l"(p));
-  return v;
-}
 __device__ __forceinline__ uint32_t word(const uint4& v, int j) {
   return j == 0 ? v.x : j == 1 ? v.y : j == 2 ? v.z : v.w;
 }
@@ -152,13 +200,63 @@ __device__ __forceinline__ void write_row(const AttnArgs& a, int t, int hq, int 
   a.out[t * a.o_st + (long)hq * D + d] = __float2bfloat16_rn(o);
 }
 
-template <bool FP8, int NT>
+// A warp's copies ahead: the codes and scales of its 16 keys of every unit of the CTA's range, in order,
+// one unit a stage.
+template <int STAGES>
+struct Ahead {
+  Walk w;
+  bool live;
+  int u, most, block, first;  // next unit; this lane's block, of unit first + lane
+  uint8_t* ring;
+  float* scales;
+
+  __device__ __forceinline__ void segment(const AttnArgs& a, int first_row, int tile_rows) {
+    live = w.next(a, first_row);
+    if (live) {
+      u = w.u0;
+      most = w.most(a, first_row, min(w.n * a.G - first_row, tile_rows));
+      first = u - 32;
+    }
+  }
+  __device__ __forceinline__ void copy(const AttnArgs& a, int stage, int warp, int lane, int first_row, int tile_rows) {
+    while (live && (u >= w.u1 || u * kUnitKeys + warp * 16 >= most)) segment(a, first_row, tile_rows);
+    if (live) {
+      if (u - first == 32) {
+        first = u;
+        const int kb = (u + lane) * kUnitKeys + warp * 16;
+        block = 0;
+        if (u + lane < w.u1 && kb < w.len) block = a.tables[w.i * a.table_ld + (kb >> a.size_log2)];
+        if (block < 0 || block >= a.num_blocks) block = 0;  // not a table of this cache
+      }
+      const long bh = (long)__shfl_sync(~0u, block, u - first) * a.Hkv + w.h;
+      const int kb = u * kUnitKeys + warp * 16;
+      const long base = ((bh << a.size_log2) + (kb & ((1 << a.size_log2) - 1))) * D + lane * 16;
+      uint8_t* to = ring + stage * kStage;
+      // four rows of 128 bytes an instruction; the 16-byte pieces of a row change places so that the
+      // reads below meet no bank twice
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int r = j * 4 + (lane >> 3), c = lane & 7;
+        copy16(to + r * D + ((c ^ ((r & 1) * 4)) << 4), a.kc + base + j * 4 * D);
+        copy16(to + kStage / 2 + r * D + ((c ^ (r & 6)) << 4), a.vc + base + j * 4 * D);
+      }
+      if (lane < 2) copy4(scales + stage * 2 + lane, (lane ? a.vs : a.ks) + bh);
+      ++u;
+    }
+    copy_commit();
+  }
+};
+
+template <bool FP8, int NT, int STAGES>
 __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) paged_attention_kernel(const AttnArgs a) {
   constexpr int ROWS = 8 * NT;
-  extern __shared__ float s_o[];  // [kWarps][rows of the tile][D]
+  extern __shared__ __align__(128) uint8_t s_ring[];  // [kWarps][STAGES][kStage], then the merge's
+  float* s_o = reinterpret_cast<float*>(s_ring + kWarps * STAGES * kStage);  // [kWarps][rows of the tile][D]
+  __shared__ float s_scales[kWarps][STAGES][2];
   __shared__ float s_m[kWarps][ROWS], s_l[kWarps][ROWS];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, tg = lane & 3;
-  const int worker = blockIdx.x, tile = blockIdx.y, Hq = a.Hkv * a.G;
+  const int worker = blockIdx.x, tile = blockIdx.y, r0 = tile * ROWS, Hq = a.Hkv * a.G;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the join may take its places; it waits for the end
 
   if (tile == 0)  // rows of no request
     for (long t = a.cu_new[a.R] + worker; t < a.T; t += gridDim.x)
@@ -166,20 +264,26 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) paged_attention_ker
         *reinterpret_cast<uint4*>(a.out + t * a.o_st + c * 8) = make_uint4(0, 0, 0, 0);
 
   const long total = (long)a.cu_units[a.R] * a.Hkv, per = (total + gridDim.x - 1) / gridDim.x;
-  long x = per * worker;
-  const long x_end = min(total, x + per);
-  while (x < x_end) {
-    const Place at = find_place(a, x);
-    const int u0 = at.u, u1 = (int)min((long)at.nu, at.u + (x_end - x));
-    x += u1 - u0;
-    const int row_t = a.cu_new[at.i], n = a.cu_new[at.i + 1] - row_t, len = a.kv_len[at.i];
-    const int r0 = tile * ROWS, rows = min(n * a.G - r0, ROWS);
-    if (rows <= 0) continue;
+  if (per * worker >= total) return;
+  Walk at;
+  at.start(a, per * worker, min(total, per * (worker + 1)), find_request(a, per * worker));
+  Ahead<STAGES> ahead;
+  ahead.w = at;
+  ahead.ring = s_ring + warp * STAGES * kStage;
+  ahead.scales = s_scales[warp][0];
+  ahead.segment(a, r0, ROWS);
+#pragma unroll
+  for (int st = 0; st < STAGES - 1; ++st) ahead.copy(a, st, warp, lane, r0, ROWS);
+  int stage = 0;
+
+  while (at.next(a, r0)) {
+    const int row_t = at.row_t, n = at.n, len = at.len, u0 = at.u0, u1 = at.u1;
+    const int rows = min(n * a.G - r0, ROWS);
 
     // queries as the B operand, scaled to f16; limits and logit factors of this lane's columns
     uint32_t qf[NT][8][2];
     float factor[NT][2];
-    int limit[NT][2], most = 0;
+    int limit[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       const int r = nt * 8 + g;
@@ -217,7 +321,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) paged_attention_ker
         limit[nt][c] = rc >= rows ? 0 : a.causal ? len - n + (r0 + rc) / a.G + 1 : len;
       }
     }
-    most = a.causal ? len - n + (r0 + rows - 1) / a.G + 1 : len;  // of the tile's rows
+    const int most = at.most(a, r0, rows);
     const int least = a.causal ? len - n + r0 / a.G + 1 : len;
 
     float o[NT][8][4] = {}, m[NT][2], l[NT][2];
@@ -230,31 +334,21 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) paged_attention_ker
       }
     float unit = 0.f;  // O is held in multiples of this
 
-    const int* table = a.tables + at.i * a.table_ld;
-    int my_block = 0;
-    float my_ks = 0.f, my_vs = 0.f;
     for (int u = u0; u < u1; ++u) {
-      if (((u - u0) & 31) == 0) {  // blocks and scales of this warp's next 32 units, one a lane
-        const int kb = (u + lane) * kUnit + warp * 16;
-        my_block = 0;
-        my_ks = my_vs = 0.f;
-        if (u + lane < u1 && kb < len) {
-          my_block = table[kb >> a.size_log2];
-          if (my_block < 0 || my_block >= a.num_blocks) my_block = 0;  // not a table of this cache
-          my_ks = a.ks[(long)my_block * a.Hkv + at.h];
-          my_vs = a.vs[(long)my_block * a.Hkv + at.h];
-        }
-      }
-      const int block = __shfl_sync(~0u, my_block, (u - u0) & 31);
-      const float ks = __shfl_sync(~0u, my_ks, (u - u0) & 31), vs = __shfl_sync(~0u, my_vs, (u - u0) & 31);
-      const int kb = u * kUnit + warp * 16;
-      if (kb >= most) continue;
-      const long base = ((((long)block * a.Hkv + at.h) << a.size_log2) + (kb & ((1 << a.size_log2) - 1))) * D;
-      const uint8_t* kp = a.kc + base + g * D + tg * 16;
-      const uint8_t* vp = a.vc + base + 2 * tg * D + g * 16;
-      const uint4 k0 = load_codes(kp), k1 = load_codes(kp + 64), k2 = load_codes(kp + 8 * D),
-                  k3 = load_codes(kp + 8 * D + 64);
-      const uint4 v0 = load_codes(vp), v1 = load_codes(vp + D), v2 = load_codes(vp + 8 * D), v3 = load_codes(vp + 9 * D);
+      const int kb = u * kUnitKeys + warp * 16;
+      if (kb >= most) break;
+      copy_wait<STAGES - 2>();
+      __syncwarp();  // this stage is there, and the stage before it was read by every lane
+      ahead.copy(a, stage == 0 ? STAGES - 1 : stage - 1, warp, lane, r0, ROWS);
+      const uint8_t* kp = s_ring + (warp * STAGES + stage) * kStage + g * D + ((tg ^ ((g & 1) * 4)) << 4);
+      const uint8_t* vp = s_ring + (warp * STAGES + stage) * kStage + kStage / 2 + 2 * tg * D + ((g ^ (2 * tg)) << 4);
+      const float ks = s_scales[warp][stage][0], vs = s_scales[warp][stage][1];
+      stage = stage == STAGES - 1 ? 0 : stage + 1;
+      const auto codes = [](const uint8_t* p) { return *reinterpret_cast<const uint4*>(p); };
+      // rows g and g + 8 of the keys (pieces tg and tg + 4), rows 2 tg, 2 tg + 1 and those 8 below of the values
+      const uint8_t* kp1 = s_ring + (kp - s_ring ^ 64);
+      const uint4 k0 = codes(kp), k1 = codes(kp1), k2 = codes(kp + 8 * D), k3 = codes(kp1 + 8 * D);
+      const uint4 v0 = codes(vp), v1 = codes(vp + D), v2 = codes(vp + 8 * D), v3 = codes(vp + 9 * D);
 
       float s[NT][4] = {};
 #pragma unroll
@@ -403,14 +497,20 @@ template <int NT>
 __global__ void __launch_bounds__(kThreads) paged_attention_join_kernel(const AttnArgs a) {
   constexpr int ROWS = 8 * NT;
   const long total = (long)a.cu_units[a.R] * a.Hkv, per = (total + gridDim.x - 1) / gridDim.x;
-  const int worker = blockIdx.x, tile = blockIdx.y;
+  const int worker = blockIdx.x, tile = blockIdx.y, r0 = tile * ROWS;
   const long x = per * worker, x_end = min(total, x + per);
-  if (x >= x_end) return;
-  const Place at = find_place(a, x);
-  if (at.u == 0 || x + (at.nu - at.u) > x_end) return;  // starts here, or goes on in the next range
-  const int row_t = a.cu_new[at.i], n = a.cu_new[at.i + 1] - row_t;
-  const int r0 = tile * ROWS, rows = min(n * a.G - r0, ROWS);
-  const int first = (int)((x - at.u) / per);
+  if (x >= x_end) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    return;
+  }
+  const int i = find_request(a, x), c0 = a.cu_units[i], cost = a.cu_units[i + 1] - c0;
+  const long in = x - (long)c0 * a.Hkv;
+  const int h = (int)(in / cost), p = (int)(in - (long)h * cost);
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // the parts are written; in every CTA, so this grid ends last
+  if (p <= kPairCost || x + (cost - p) > x_end) return;  // starts here, or goes on in the next range
+  const int row_t = a.cu_new[i], n = a.cu_new[i + 1] - row_t;
+  const int rows = min(n * a.G - r0, ROWS);
+  const int first = (int)((x - p + kPairCost) / per);
   const auto place = [&](int w) {  // the first worker may start with the pair or before it
     return a.part + ((long)(2 * w + (w == first ? 1 : 0)) * gridDim.y + tile) * ROWS * (D + 2);
   };
@@ -426,35 +526,47 @@ __global__ void __launch_bounds__(kThreads) paged_attention_join_kernel(const At
       sum += p[D + 1] * f;
       out += p[d] * f;
     }
-    write_row(a, row_t + (r0 + r) / a.G, at.h * a.G + (r0 + r) % a.G, d, sum == 0.f ? 0.f : out / sum);
+    write_row(a, row_t + (r0 + r) / a.G, h * a.G + (r0 + r) % a.G, d, sum == 0.f ? 0.f : out / sum);
   }
 }
 
-template <bool FP8, int NT>
+template <bool FP8, int NT, int STAGES>
 void launch(AttnArgs a, int max_rows, const at::TensorOptions& opts, cudaStream_t stream) {
   constexpr int ROWS = 8 * NT;
   const int tiles = (max_rows + ROWS - 1) / ROWS;
   TORCH_CHECK(tiles <= 65535, "paged_attention: too many new tokens for one request");
-  const int smem = kWarps * ROWS * D * 4;
-  C10_CUDA_CHECK(ensure_dynamic_smem((const void*)paged_attention_kernel<FP8, NT>, smem));
+  const int smem = kWarps * (STAGES * kStage + std::min(max_rows, ROWS) * D * 4);
+  C10_CUDA_CHECK(ensure_dynamic_smem((const void*)paged_attention_kernel<FP8, NT, STAGES>,
+                                     kWarps * (STAGES * kStage + ROWS * D * 4)));
   const int workers = device_sm_count() * (NT == 1 ? 2 : 1);
   const at::Tensor part = at::empty({2L * workers * tiles * ROWS * (D + 2)}, opts.dtype(at::kFloat));
   a.part = part.data_ptr<float>();
   const dim3 grid(workers, tiles);
-  paged_attention_kernel<FP8, NT><<<grid, kThreads, smem, stream>>>(a);
+  paged_attention_kernel<FP8, NT, STAGES><<<grid, kThreads, smem, stream>>>(a);
   C10_CUDA_KERNEL_LAUNCH_CHECK();
-  paged_attention_join_kernel<NT><<<grid, kThreads, 0, stream>>>(a);
-  C10_CUDA_KERNEL_LAUNCH_CHECK();
+  // the join is launched while the first kernel runs and waits for its end itself
+  cudaLaunchConfig_t config{};
+  config.gridDim = grid;
+  config.blockDim = dim3(kThreads);
+  config.stream = stream;
+  cudaLaunchAttribute early{};
+  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early.val.programmaticStreamSerializationAllowed = 1;
+  config.attrs = &early;
+  config.numAttrs = 1;
+  C10_CUDA_CHECK(cudaLaunchKernelEx(&config, paged_attention_join_kernel<NT>, a));
 }
 
 template <bool FP8>
 void launch_rows(const AttnArgs& a, int max_rows, const at::TensorOptions& opts, cudaStream_t stream) {
-  if (max_rows <= 8)
-    launch<FP8, 1>(a, max_rows, opts, stream);
+  if (max_rows <= 4)
+    launch<FP8, 1, 3>(a, max_rows, opts, stream);
+  else if (max_rows <= 8)
+    launch<FP8, 1, 2>(a, max_rows, opts, stream);
   else if (max_rows <= 16)
-    launch<FP8, 2>(a, max_rows, opts, stream);
+    launch<FP8, 2, 4>(a, max_rows, opts, stream);
   else
-    launch<FP8, 4>(a, max_rows, opts, stream);
+    launch<FP8, 4, 3>(a, max_rows, opts, stream);
 }
 
 }  // namespace
@@ -491,7 +603,6 @@ at::Tensor paged_attention(const at::Tensor& query, const at::Tensor& keys, cons
   TORCH_CHECK(meta.device() == keys.device() && meta.scalar_type() == at::kInt && meta.is_contiguous() &&
                   meta.numel() == 3 * R + 3,
               "paged_attention: a step of these tables");
-  TORCH_CHECK(paged_unit_keys() == kUnit, "paged_attention: unit of the step");
   c10::cuda::CUDAGuard guard(keys.device());
   const at::Tensor out = at::empty({T, query.size(1), D}, query.options());
   if (T == 0) return out;

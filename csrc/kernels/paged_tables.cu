@@ -24,6 +24,7 @@
 
 #include "common.cuh"
 #include "device_setup.h"
+#include "paged.h"
 
 namespace hrm {
 namespace {
@@ -31,7 +32,6 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr int kMaxRequests = 8192;  // three prefix arrays of this many int32 in shared memory
-constexpr int kUnitKeys = 128;      // keys of one unit of attention work (paged_attention.cu)
 
 // status codes; the Python side names them
 enum StepStatus : int { kStepOk = 0, kStepPool = 1, kStepRows = 2, kStepLong = 3, kStepNegative = 4, kStepMaxNew = 5 };
@@ -133,7 +133,7 @@ __global__ void __launch_bounds__(kThreads) paged_step_kernel(const StepArgs a) 
       mine.a += n;
       mine.b += blocks(len + n) - blocks(len);
       mine.c += blocks(len + n) - (len >> a.size_log2);
-      mine.d += (len + n + kUnitKeys - 1) / kUnitKeys;
+      mine.d += (len + n + kUnitKeys - 1) / kUnitKeys + kPairCost;
     }
   }
   const Sums first = block_exclusive(mine, total);
@@ -165,7 +165,7 @@ __global__ void __launch_bounds__(kThreads) paged_step_kernel(const StepArgs a) 
       at.a += n;
       at.b += blocks(len + n) - blocks(len);
       at.c += blocks(len + n) - (len >> a.size_log2);
-      at.d += (len + n + kUnitKeys - 1) / kUnitKeys;
+      at.d += (len + n + kUnitKeys - 1) / kUnitKeys + kPairCost;
     }
   }
   const int used = failed ? 0 : (int)total.a;
@@ -279,7 +279,6 @@ int log2_of(int64_t v) {
 }  // namespace
 
 int64_t paged_max_requests() { return kMaxRequests; }
-int64_t paged_unit_keys() { return kUnitKeys; }
 
 // One step: see the head of this file. Returns int32 tensors: slots and positions [rows]; runs
 // [max_runs, 4] (block, first offset, tokens, first row); meta, which is cu_new [R + 1], cu_units

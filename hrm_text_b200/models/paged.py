@@ -12,7 +12,7 @@ from typing import Optional
 import torch
 from torch import Tensor
 
-from ..ops.paged import UNIT_KEYS, BlockTables, PagedKV8, StepPlan, paged_append, paged_attention
+from ..ops.paged import PAIR_COST, UNIT_KEYS, BlockTables, PagedKV8, StepPlan, paged_append, paged_attention
 
 QMAX = {torch.int8: 127.0, torch.float8_e4m3fn: 448.0}
 
@@ -54,7 +54,7 @@ def step_reference(tables: BlockTables, new_tokens: Tensor, plan: StepPlan) -> N
             plan.positions[row + done:row + done + take] = pos + torch.arange(take, dtype=torch.int32)
             done += take
         row += n
-        units += -(-(length + n) // UNIT_KEYS) if n else 0
+        units += -(-(length + n) // UNIT_KEYS) + PAIR_COST if n else 0
     plan.cu_new[-1], plan.cu_units[-1], plan.num_runs[0] = row, units, len(runs)
     if runs:
         plan.runs[:len(runs)] = torch.tensor(runs, dtype=torch.int32)
