@@ -13,29 +13,31 @@
 // there; the parts of a pair that spans CTAs go to a workspace and a second kernel joins them in
 // order (no atomics: the same inputs give the same bits).
 //
-// In a CTA each of 8 warps takes 16 keys of a unit and keeps its own running maximum, sum and
-// output for up to 8 * NT query rows (G query heads times the request's new tokens); the
-// warps are merged through shared memory once per pair. Each warp copies its own codes ahead into
-// its own ring of shared memory (cp.async, 4 KB a stage), across the ends of pairs, so that it
-// waits for no other warp and a pair's first loads run under the work before it.
-// A warp's 16 keys are
+// In a CTA each of 4 warps takes 32 keys of a unit and keeps its own running maximum, sum and
+// output for up to 8 * NT query rows (G query heads times the request's new tokens; requests with
+// more rows take several tiles). The warps are merged through shared memory once per pair. Each
+// warp copies its own codes ahead into its own ring of shared memory (cp.async, 8 KB a stage), across
+// the ends of pairs, so that it waits for no other warp and a pair's first loads run under the
+// work before it. 16 of a warp's keys are
 //   S^T [16 keys x 8 rows] = C [16 x 128] Q^T,   O^T [128 dims x 8 rows] += C'^T [128 x 16] P^T
 // in mma.m16n8k16 with the keys as the M side: 8 rows, the smallest N, waste the least of a
-// matrix instruction on the one or few rows a decode step has. The kernel is bound by reading the
-// codes (256 bytes a key and head for 4 * 128 * rows flops), so warp-level matrix instructions
-// on codes converted in registers are far from their limit:
+// matrix instruction on the one or few rows a decode step has. The kernel reads 256 bytes a key
+// and head for 4 * 128 * rows flops, so warp-level matrix instructions are far from their limit; what
+// counts is how few instructions a byte of codes takes:
 //   * the k index of S = C Q^T may be permuted as one likes if Q is permuted alike, so a lane
 //     owns 32 dims of two keys as four 16-byte words, and a 32-bit word of codes is the lane's
 //     part of one k step;
 //   * the m index of O^T likewise: a lane owns 16 dims of four keys, pairs of keys are
 //     interleaved by byte permutes before they are widened;
 //   * P^T is S^T transposed 8x8 by movmatrix.
-// Codes are exact in f16 (int8: 1024 + 128 + c by a byte permute, minus 1152; e4m3: one cvt).
-// Queries are scaled by a power of two to a row maximum in [1, 2) before they are rounded to f16:
-// a bf16 value keeps all its bits unless it is 2^-14 of the row's largest. P is rounded to f16 (11
-// bits, against 8 of bf16), sums stay fp32. The key scale multiplies the fp32 score; the value
-// scale is kept as the unit of the accumulators: O is held in multiples of the current
-// block's scale and multiplied by (old unit / new unit) where it changes.
+// Codes are exact in f16: e4m3 by one cvt, int8 as 1152 + c by one byte permute. Values subtract the
+// 1152; for keys the accumulators start at -1152 sum q instead. Queries are scaled by a power of two
+// to a row maximum in [1, 2) before they are rounded to f16: a bf16 value keeps all its bits
+// unless it is 2^-14 of the row's largest. P is rounded to f16 (11 bits, against 8 of bf16), sums
+// stay fp32. The key scale multiplies the fp32 score. O is held in multiples of a unit, the
+// largest value scale met: P is multiplied by (scale / unit) before it is rounded, and where that
+// leaves [2^-10, 1] the unit becomes this block's scale and O is rescaled, so that small values
+// keep their bits beside large ones.
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <cuda_fp16.h>
@@ -49,11 +51,16 @@ namespace hrm {
 namespace {
 
 constexpr int D = 128;
-constexpr int kWarps = 8;
+constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
-constexpr int kStage = 2 * 16 * D;  // bytes of a warp's 16 keys: codes of keys, then of values
-constexpr float kLazy = 8.f;        // a running maximum may lag by 2^8: P stays below 256 in f16
-constexpr float kMinUnit = 0x1p-64f;  // a unit is at least this part of the one before it
+constexpr int kJoin = 256;  // threads of the joining kernel
+constexpr int kKeys = kUnitKeys / kWarps;  // a warp's keys of a unit: two halves of 16
+constexpr int kHalf = 2 * 16 * D;          // bytes of 16 keys: codes of keys, then of values
+constexpr int kStage = 2 * kHalf;
+constexpr int kStages = 2;      // one is read while the other is filled
+constexpr int kPart = D + 4;    // floats of a row's part, in whole 16 bytes
+constexpr float kLazy = 8.f;    // a running maximum may lag by 2^8: P stays below 256 in f16
+constexpr float kLeast = 0x1p-10f, kFar = 0x1p-60f;  // P times something between these changes the unit
 
 struct AttnArgs {
   const __nv_bfloat16* q;
@@ -73,18 +80,18 @@ struct AttnArgs {
   long g_st, g_sh;
   __nv_bfloat16* out;  // [T, Hq, 128]
   long o_st;
-  float* part;  // [2 * workers][tiles][8 * NT][130]: output, maximum, sum
+  float* part;  // [2 * workers][tiles][8 * NT][kPart]: output, maximum, sum
 };
 
 // The request whose part of the costs laid end to end holds position `x`; every thread of the CTA
 // calls it.
 __device__ __forceinline__ int find_request(const AttnArgs& a, long x) {
   int i = 0;
-  for (int base = 0; base < a.R; base += kThreads) {
+  for (int base = 0; base < a.R; base += (int)blockDim.x) {
     const int j = base + (int)threadIdx.x;
     const int c = __syncthreads_count(j < a.R && (long)a.cu_units[j + 1] * a.Hkv <= x);
     i += c;
-    if (c < kThreads) break;
+    if (c < (int)blockDim.x) break;
   }
   return i;
 }
@@ -141,34 +148,23 @@ __device__ __forceinline__ void copy4(void* smem, const void* global) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(smem)), "l"(global) : "memory");
 }
 __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void copy_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
+__device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group 0;" ::: "memory"); }
 
-template <bool FP8>
-__device__ __forceinline__ uint32_t widen(uint32_t two) {  // two codes in the low 16 bits -> f16x2
+// Two codes, in bytes 0 and 1 (HI: 2 and 3) of a word, as f16x2: e4m3 themselves; int8, given as code + 128,
+// as 1024 + that, less 1152 for values (EXACT) and not for keys.
+template <bool FP8, bool HI, bool EXACT>
+__device__ __forceinline__ uint32_t widen(uint32_t w) {
+  uint32_t r;
   if constexpr (FP8) {
-    uint32_t r;
-    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"((unsigned short)two));
-    return r;
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"((unsigned short)(HI ? w >> 16 : w)));
   } else {
-    uint32_t r = __byte_perm(two, 0x64646464u, 0x4140);
-    const __half2 bias = __half2half2(__ushort_as_half(0x6480));  // 1152
-    const __half2 v = __hsub2(*reinterpret_cast<__half2*>(&r), bias);
-    return *reinterpret_cast<const uint32_t*>(&v);
+    r = __byte_perm(w, 0x64646464u, HI ? 0x4342 : 0x4140);
+    if constexpr (EXACT) {
+      const __half2 v = __hsub2(*reinterpret_cast<__half2*>(&r), __half2half2(__ushort_as_half(0x6480)));
+      r = *reinterpret_cast<const uint32_t*>(&v);
+    }
   }
-}
-template <bool FP8>
-__device__ __forceinline__ uint32_t widen_hi(uint32_t w) {  // the codes in the high 16 bits
-  if constexpr (FP8) {
-    return widen<true>(w >> 16);
-  } else {
-    uint32_t r = __byte_perm(w, 0x64646464u, 0x4342);
-    const __half2 bias = __half2half2(__ushort_as_half(0x6480));
-    const __half2 v = __hsub2(*reinterpret_cast<__half2*>(&r), bias);
-    return *reinterpret_cast<const uint32_t*>(&v);
-  }
+  return r;
 }
 // int8 codes are widened from code + 128
 template <bool FP8>
@@ -200,60 +196,67 @@ __device__ __forceinline__ void write_row(const AttnArgs& a, int t, int hq, int 
   a.out[t * a.o_st + (long)hq * D + d] = __float2bfloat16_rn(o);
 }
 
-// A warp's copies ahead: the codes and scales of its 16 keys of every unit of the CTA's range, in order,
+// A warp's copies ahead: the codes and scales of its keys of every unit of the CTA's range, in order,
 // one unit a stage.
-template <int STAGES>
 struct Ahead {
   Walk w;
   bool live;
-  int u, most, block, first;  // next unit; this lane's block, of unit first + lane
+  int u, most, first, block;  // next unit; this lane's block: of unit first + lane / 2, half lane % 2
   uint8_t* ring;
-  float* scales;
+  float* scales;  // [kStages][2 halves][keys, values]
 
   __device__ __forceinline__ void segment(const AttnArgs& a, int first_row, int tile_rows) {
     live = w.next(a, first_row);
     if (live) {
       u = w.u0;
       most = w.most(a, first_row, min(w.n * a.G - first_row, tile_rows));
-      first = u - 32;
+      first = u - 16;
     }
   }
   __device__ __forceinline__ void copy(const AttnArgs& a, int stage, int warp, int lane, int first_row, int tile_rows) {
-    while (live && (u >= w.u1 || u * kUnitKeys + warp * 16 >= most)) segment(a, first_row, tile_rows);
+    while (live && (u >= w.u1 || u * kUnitKeys + warp * kKeys >= most)) segment(a, first_row, tile_rows);
     if (live) {
-      if (u - first == 32) {
+      if (u - first == 16) {
         first = u;
-        const int kb = (u + lane) * kUnitKeys + warp * 16;
+        // a half after the last token takes the block, and so the scales, of the half before it
+        const int kb = (u + (lane >> 1)) * kUnitKeys + warp * kKeys + (lane & 1) * 16;
         block = 0;
-        if (u + lane < w.u1 && kb < w.len) block = a.tables[w.i * a.table_ld + (kb >> a.size_log2)];
+        if (u + (lane >> 1) < w.u1) block = a.tables[w.i * a.table_ld + (min(kb, w.len - 1) >> a.size_log2)];
         if (block < 0 || block >= a.num_blocks) block = 0;  // not a table of this cache
       }
-      const long bh = (long)__shfl_sync(~0u, block, u - first) * a.Hkv + w.h;
-      const int kb = u * kUnitKeys + warp * 16;
-      const long base = ((bh << a.size_log2) + (kb & ((1 << a.size_log2) - 1))) * D + lane * 16;
-      uint8_t* to = ring + stage * kStage;
-      // four rows of 128 bytes an instruction; the 16-byte pieces of a row change places so that the
-      // reads below meet no bank twice
+      // lane's row of each four and its 16-byte piece; the pieces of a row change places so that the
+      // reads meet no bank twice: by 4 in odd rows of keys, by (row & 6) in rows of values
+      const int q = lane >> 3, c = lane & 7;
+      uint8_t* kto = ring + stage * kStage + q * D + ((c ^ ((q & 1) * 4)) << 4);
+      uint8_t* vto = ring + stage * kStage + kHalf / 2 + q * D + ((c ^ (q & 2)) << 4);
+      const int odd = ((c ^ (q & 2) ^ 4) - (c ^ (q & 2))) * 16;  // to the place in rows 4 to 7 and 12 to 15
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int r = j * 4 + (lane >> 3), c = lane & 7;
-        copy16(to + r * D + ((c ^ ((r & 1) * 4)) << 4), a.kc + base + j * 4 * D);
-        copy16(to + kStage / 2 + r * D + ((c ^ (r & 6)) << 4), a.vc + base + j * 4 * D);
+      for (int half = 0; half < 2; ++half) {
+        const int kb = u * kUnitKeys + warp * kKeys + half * 16;
+        const long bh = (long)__shfl_sync(~0u, block, 2 * (u - first) + half) * a.Hkv + w.h;
+        const long base = ((bh << a.size_log2) + (kb & ((1 << a.size_log2) - 1))) * D + lane * 16;
+        const uint8_t *kp = a.kc + base, *vp = a.vc + base;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          copy16(kto + half * kHalf + j * 4 * D, kp + j * 4 * D);
+          copy16(vto + half * kHalf + j * 4 * D + (j & 1) * odd, vp + j * 4 * D);
+        }
+        if (lane < 2) copy4(scales + stage * 4 + half * 2 + lane, (lane ? a.vs : a.ks) + bh);
       }
-      if (lane < 2) copy4(scales + stage * 2 + lane, (lane ? a.vs : a.ks) + bh);
       ++u;
     }
     copy_commit();
   }
 };
 
-template <bool FP8, int NT, int STAGES>
-__global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) paged_attention_kernel(const AttnArgs a) {
+template <bool FP8, int NT>
+__global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) paged_attention_kernel(const AttnArgs a) {
   constexpr int ROWS = 8 * NT;
-  extern __shared__ __align__(128) uint8_t s_ring[];  // [kWarps][STAGES][kStage], then the merge's
-  float* s_o = reinterpret_cast<float*>(s_ring + kWarps * STAGES * kStage);  // [kWarps][rows of the tile][D]
-  __shared__ float s_scales[kWarps][STAGES][2];
+  static_assert(ROWS * D * 4 <= kStage, "a stage holds a warp's part of the merge");
+  extern __shared__ __align__(128) uint8_t s_ring[];  // [kWarps][kStages][kStage]
+  __shared__ __align__(16) float s_scales[kWarps][kStages][2][2];
   __shared__ float s_m[kWarps][ROWS], s_l[kWarps][ROWS];
+  __shared__ int s_part[kWarps];  // where in s_ring a warp's part of the merge is, -1: it has none
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, tg = lane & 3;
   const int worker = blockIdx.x, tile = blockIdx.y, r0 = tile * ROWS, Hq = a.Hkv * a.G;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the join may take its places; it waits for the end
@@ -267,14 +270,19 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) paged_attention_ker
   if (per * worker >= total) return;
   Walk at;
   at.start(a, per * worker, min(total, per * (worker + 1)), find_request(a, per * worker));
-  Ahead<STAGES> ahead;
+  Ahead ahead;
   ahead.w = at;
-  ahead.ring = s_ring + warp * STAGES * kStage;
-  ahead.scales = s_scales[warp][0];
+  ahead.ring = s_ring + warp * kStages * kStage;
+  ahead.scales = s_scales[warp][0][0];
   ahead.segment(a, r0, ROWS);
-#pragma unroll
-  for (int st = 0; st < STAGES - 1; ++st) ahead.copy(a, st, warp, lane, r0, ROWS);
+  ahead.copy(a, 0, warp, lane, r0, ROWS);
   int stage = 0;
+  // this lane's pieces: rows g and g + 8 of the keys, pieces tg and tg + 4; rows 2 tg, 2 tg + 1 and those 8
+  // below of the values, piece g
+  const uint8_t* k_lane = ahead.ring + g * D + ((tg ^ ((g & 1) * 4)) << 4);
+  const int k_more = ((tg ^ ((g & 1) * 4) ^ 4) - (tg ^ ((g & 1) * 4))) * 16;
+  const uint8_t* v_lane = ahead.ring + kHalf / 2 + 2 * tg * D + ((g ^ (2 * tg)) << 4);
+  const auto codes = [](const uint8_t* p) { return *reinterpret_cast<const uint4*>(p); };
 
   while (at.next(a, r0)) {
     const int row_t = at.row_t, n = at.n, len = at.len, u0 = at.u0, u1 = at.u1;
@@ -282,7 +290,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) paged_attention_ker
 
     // queries as the B operand, scaled to f16; limits and logit factors of this lane's columns
     uint32_t qf[NT][8][2];
-    float factor[NT][2];
+    float factor[NT][2], start[NT][2];
     int limit[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
@@ -307,16 +315,24 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) paged_attention_ker
       // 2^-e with e the exponent of the largest magnitude (within what a float can hold)
       const int e = min(126, max(-126, (int)(top >> 7) - 127));
       const float down = __uint_as_float((uint32_t)(127 - e) << 23);
+      float sum = 0.f;
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const float2 lo = unpack_bf16x2(word(raw[j / 2], (j & 1) * 2)), hi = unpack_bf16x2(word(raw[j / 2], (j & 1) * 2 + 1));
-        qf[nt][j][0] = pack_f16x2(lo.x * down, lo.y * down);
-        qf[nt][j][1] = pack_f16x2(hi.x * down, hi.y * down);
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const float2 v = unpack_bf16x2(word(raw[j / 2], (j & 1) * 2 + c));
+          qf[nt][j][c] = pack_f16x2(v.x * down, v.y * down);
+          const float2 w = __half22float2(*reinterpret_cast<const __half2*>(&qf[nt][j][c]));
+          sum += w.x + w.y;
+        }
       }
+      sum += __shfl_xor_sync(~0u, sum, 1);
+      sum += __shfl_xor_sync(~0u, sum, 2);
       const float up = __uint_as_float((uint32_t)(127 + e) << 23) * a.scale_log2;
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         factor[nt][c] = __shfl_sync(~0u, up, (2 * tg + c) * 4);
+        start[nt][c] = FP8 ? 0.f : -1152.f * __shfl_sync(~0u, sum, (2 * tg + c) * 4);
         const int rc = nt * 8 + 2 * tg + c;
         limit[nt][c] = rc >= rows ? 0 : a.causal ? len - n + (r0 + rc) / a.G + 1 : len;
       }
@@ -324,122 +340,155 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) paged_attention_ker
     const int most = at.most(a, r0, rows);
     const int least = a.causal ? len - n + r0 / a.G + 1 : len;
 
-    float o[NT][8][4] = {}, m[NT][2], l[NT][2];
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        m[nt][c] = -INFINITY;
-        l[nt][c] = 0.f;
-      }
-    float unit = 0.f;  // O is held in multiples of this
+    float o[NT][8][4] = {}, m[NT][2] = {}, l[NT][2] = {};
+    int none = (1 << 2 * NT) - 1;            // columns that have no maximum yet
+    float unit = 0.f, inv_unit = INFINITY;  // O is held in multiples of this
+    int last = -1;                          // the stage read last
 
     for (int u = u0; u < u1; ++u) {
-      const int kb = u * kUnitKeys + warp * 16;
+      const int kb = u * kUnitKeys + warp * kKeys;
       if (kb >= most) break;
-      copy_wait<STAGES - 2>();
-      __syncwarp();  // this stage is there, and the stage before it was read by every lane
-      ahead.copy(a, stage == 0 ? STAGES - 1 : stage - 1, warp, lane, r0, ROWS);
-      const uint8_t* kp = s_ring + (warp * STAGES + stage) * kStage + g * D + ((tg ^ ((g & 1) * 4)) << 4);
-      const uint8_t* vp = s_ring + (warp * STAGES + stage) * kStage + kStage / 2 + 2 * tg * D + ((g ^ (2 * tg)) << 4);
-      const float ks = s_scales[warp][stage][0], vs = s_scales[warp][stage][1];
-      stage = stage == STAGES - 1 ? 0 : stage + 1;
-      const auto codes = [](const uint8_t* p) { return *reinterpret_cast<const uint4*>(p); };
-      // rows g and g + 8 of the keys (pieces tg and tg + 4), rows 2 tg, 2 tg + 1 and those 8 below of the values
-      const uint8_t* kp1 = s_ring + (kp - s_ring ^ 64);
-      const uint4 k0 = codes(kp), k1 = codes(kp1), k2 = codes(kp + 8 * D), k3 = codes(kp1 + 8 * D);
-      const uint4 v0 = codes(vp), v1 = codes(vp + D), v2 = codes(vp + 8 * D), v3 = codes(vp + 9 * D);
+      copy_wait();
+      __syncwarp();  // this stage is there, and the other one was read by every lane
+      ahead.copy(a, stage ^ 1, warp, lane, r0, ROWS);
+      last = stage;
+      const float4 scale = *reinterpret_cast<const float4*>(s_scales[warp][stage][0]);  // halves: keys, values
+      const uint8_t *kp = k_lane + stage * kStage, *vp = v_lane + stage * kStage;
+      stage ^= 1;
 
-      float s[NT][4] = {};
+      float s[2][NT][4];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const uint32_t lo = biased<FP8>(word(j < 4 ? k0 : k1, j & 3)), hi = biased<FP8>(word(j < 4 ? k2 : k3, j & 3));
-        const uint32_t a0 = widen<FP8>(lo), a2 = widen_hi<FP8>(lo), a1 = widen<FP8>(hi), a3 = widen_hi<FP8>(hi);
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) mma16816(s[nt], a0, a1, a2, a3, qf[nt][j][0], qf[nt][j][1]);
-      }
-
-      bool raise = false;
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        const float f0 = factor[nt][0] * ks, f1 = factor[nt][1] * ks;
-        s[nt][0] *= f0;
-        s[nt][1] *= f1;
-        s[nt][2] *= f0;
-        s[nt][3] *= f1;
-        if (kb + 16 > least) {
-          if (kb + g >= limit[nt][0]) s[nt][0] = -INFINITY;
-          if (kb + g >= limit[nt][1]) s[nt][1] = -INFINITY;
-          if (kb + g + 8 >= limit[nt][0]) s[nt][2] = -INFINITY;
-          if (kb + g + 8 >= limit[nt][1]) s[nt][3] = -INFINITY;
-        }
-        raise |= fmaxf(s[nt][0], s[nt][2]) > m[nt][0] + kLazy || fmaxf(s[nt][1], s[nt][3]) > m[nt][1] + kLazy;
-      }
-      // accumulators to the new block's unit, and under the new maximum where one has risen
-      const float next = vs == 0.f ? unit : fmaxf(vs, unit * kMinUnit) + (vs - vs);  // NaN stays NaN
-      const float ratio = next == unit ? 1.f : unit / next;
-      const float shrink = vs == next || vs == 0.f ? 1.f : vs / next;
-      unit = next;
-      raise = __any_sync(~0u, raise);
-      if (raise || ratio != 1.f) {
+      for (int half = 0; half < 2; ++half) {
+        const uint4 k0 = codes(kp + half * kHalf), k1 = codes(kp + half * kHalf + k_more),
+                    k2 = codes(kp + half * kHalf + 8 * D), k3 = codes(kp + half * kHalf + 8 * D + k_more);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          float f[2] = {ratio, ratio};
-          if (raise) {
+          s[half][nt][0] = s[half][nt][2] = start[nt][0];
+          s[half][nt][1] = s[half][nt][3] = start[nt][1];
+        }
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-              float top = fmaxf(s[nt][c], s[nt][c + 2]);
-              top = fmaxf(top, __shfl_xor_sync(~0u, top, 4));
-              top = fmaxf(top, __shfl_xor_sync(~0u, top, 8));
-              top = fmaxf(top, __shfl_xor_sync(~0u, top, 16));
-              const float now = fmaxf(m[nt][c], top);
-              const float alpha = now == m[nt][c] ? 1.f : fast_exp2(m[nt][c] - now);
-              m[nt][c] = now;
-              l[nt][c] *= alpha;
-              f[c] *= alpha;
+        for (int j = 0; j < 8; ++j) {
+          const uint32_t lo = biased<FP8>(word(j < 4 ? k0 : k1, j & 3)), hi = biased<FP8>(word(j < 4 ? k2 : k3, j & 3));
+          const uint32_t a0 = widen<FP8, false, false>(lo), a2 = widen<FP8, true, false>(lo);
+          const uint32_t a1 = widen<FP8, false, false>(hi), a3 = widen<FP8, true, false>(hi);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) mma16816(s[half][nt], a0, a1, a2, a3, qf[nt][j][0], qf[nt][j][1]);
+        }
+      }
+
+      // scores under the running maximum, which moves when one passes it by kLazy, and to a first one
+      bool raise = none != 0;
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const float ks = half ? scale.z : scale.x;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          const float f[2] = {factor[nt][0] * ks, factor[nt][1] * ks};
+#pragma unroll
+          for (int c = 0; c < 4; ++c) s[half][nt][c] = fmaf(s[half][nt][c], f[c & 1], -m[nt][c & 1]);
+        }
+      }
+      if (kb + kKeys > least) {
+#pragma unroll
+        for (int half = 0; half < 2; ++half)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+              if (kb + half * 16 + g + (c >> 1) * 8 >= limit[nt][c & 1]) s[half][nt][c] = -INFINITY;
+      }
+      float up[NT][2];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          up[nt][c] = fmaxf(fmaxf(s[0][nt][c], s[0][nt][c + 2]), fmaxf(s[1][nt][c], s[1][nt][c + 2]));
+          raise |= up[nt][c] > kLazy;
+        }
+      if (__any_sync(~0u, raise)) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          float alpha[2];
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            float by = up[nt][c];
+            by = fmaxf(by, __shfl_xor_sync(~0u, by, 4));
+            by = fmaxf(by, __shfl_xor_sync(~0u, by, 8));
+            by = fmaxf(by, __shfl_xor_sync(~0u, by, 16));
+            const int bit = 1 << (nt * 2 + c);
+            alpha[c] = 1.f;
+            if (none & bit ? by > -INFINITY : by > 0.f) {
+              if (!(none & bit)) alpha[c] = fast_exp2(-by);
+              none &= ~bit;
+              m[nt][c] += by;
+              l[nt][c] *= alpha[c];
+#pragma unroll
+              for (int half = 0; half < 2; ++half) {
+                s[half][nt][c] -= by;
+                s[half][nt][c + 2] -= by;
+              }
             }
           }
 #pragma unroll
           for (int mt = 0; mt < 8; ++mt) {
-            o[nt][mt][0] *= f[0];
-            o[nt][mt][1] *= f[1];
-            o[nt][mt][2] *= f[0];
-            o[nt][mt][3] *= f[1];
+            o[nt][mt][0] *= alpha[0];
+            o[nt][mt][1] *= alpha[1];
+            o[nt][mt][2] *= alpha[0];
+            o[nt][mt][3] *= alpha[1];
           }
         }
       }
-      uint32_t pb[NT][2];
+
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        const float m0 = m[nt][0] == -INFINITY ? 0.f : m[nt][0], m1 = m[nt][1] == -INFINITY ? 0.f : m[nt][1];
-        float p0 = fast_exp2(s[nt][0] - m0), p1 = fast_exp2(s[nt][1] - m1);
-        float p2 = fast_exp2(s[nt][2] - m0), p3 = fast_exp2(s[nt][3] - m1);
-        l[nt][0] += p0 + p2;
-        l[nt][1] += p1 + p3;
-        if (shrink != 1.f) {
-          p0 *= shrink;
-          p1 *= shrink;
-          p2 *= shrink;
-          p3 *= shrink;
+      for (int half = 0; half < 2; ++half) {
+        const float vs = half ? scale.w : scale.y;
+        const bool any = vs != 0.f && kb + half * 16 < most;  // else P or V is zero
+        float ratio = any ? vs * inv_unit : 0.f;
+        if (any && (!(ratio <= 1.f) || (ratio < kLeast && ratio > kFar))) {
+          const float to = unit / vs;
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int mt = 0; mt < 8; ++mt)
+#pragma unroll
+              for (int c = 0; c < 4; ++c) o[nt][mt][c] *= to;
+          unit = vs;
+          inv_unit = 1.f / vs;
+          ratio = 1.f;
         }
-        pb[nt][0] = transpose8x8(pack_f16x2(p0, p1));
-        pb[nt][1] = transpose8x8(pack_f16x2(p2, p3));
-      }
+        uint32_t pb[NT][2];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const uint32_t w0 = biased<FP8>(word(v0, j)), w1 = biased<FP8>(word(v1, j)), w2 = biased<FP8>(word(v2, j)),
-                       w3 = biased<FP8>(word(v3, j));
+        for (int nt = 0; nt < NT; ++nt) {
+          float p[4];
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {  // two of the word's four dims
-          const uint32_t lo = __byte_perm(w0, w1, half ? 0x7362 : 0x5140), hi = __byte_perm(w2, w3, half ? 0x7362 : 0x5140);
-          const uint32_t a0 = widen<FP8>(lo), a1 = widen_hi<FP8>(lo), a2 = widen<FP8>(hi), a3 = widen_hi<FP8>(hi);
+          for (int c = 0; c < 4; ++c) p[c] = fast_exp2(s[half][nt][c]);
+          l[nt][0] += p[0] + p[2];
+          l[nt][1] += p[1] + p[3];
+          pb[nt][0] = transpose8x8(pack_f16x2(p[0] * ratio, p[1] * ratio));
+          pb[nt][1] = transpose8x8(pack_f16x2(p[2] * ratio, p[3] * ratio));
+        }
+        const uint4 v0 = codes(vp + half * kHalf), v1 = codes(vp + half * kHalf + D), v2 = codes(vp + half * kHalf + 8 * D),
+                    v3 = codes(vp + half * kHalf + 9 * D);
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) mma16816(o[nt][2 * j + half], a0, a1, a2, a3, pb[nt][0], pb[nt][1]);
+        for (int j = 0; j < 4; ++j) {
+          const uint32_t w0 = biased<FP8>(word(v0, j)), w1 = biased<FP8>(word(v1, j)), w2 = biased<FP8>(word(v2, j)),
+                         w3 = biased<FP8>(word(v3, j));
+#pragma unroll
+          for (int two = 0; two < 2; ++two) {  // two of the word's four dims
+            const uint32_t lo = __byte_perm(w0, w1, two ? 0x7362 : 0x5140), hi = __byte_perm(w2, w3, two ? 0x7362 : 0x5140);
+            const uint32_t a0 = widen<FP8, false, true>(lo), a1 = widen<FP8, true, true>(lo);
+            const uint32_t a2 = widen<FP8, false, true>(hi), a3 = widen<FP8, true, true>(hi);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) mma16816(o[nt][2 * j + two], a0, a1, a2, a3, pb[nt][0], pb[nt][1]);
+          }
         }
       }
     }
 
-    // the warps' parts: this lane has dims 16 g + 2 mt (+ 1) of rows 2 tg and 2 tg + 1 of each 8
+    // the warps' parts, each in the stage that its warp read last: this lane has dims 16 g + 2 mt (+ 1) of
+    // rows 2 tg and 2 tg + 1 of each 8
+    __syncwarp();
+    float* mine = reinterpret_cast<float*>(ahead.ring + max(last, 0) * kStage);
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -449,42 +498,46 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) paged_attention_ker
         sum += __shfl_xor_sync(~0u, sum, 8);
         sum += __shfl_xor_sync(~0u, sum, 16);
         const int r = nt * 8 + 2 * tg + c;
-        if (r < rows) {
+        if (r < rows && last >= 0) {
           if (g == 0) {
-            s_m[warp][r] = m[nt][c];
+            s_m[warp][r] = none >> (nt * 2 + c) & 1 ? -INFINITY : m[nt][c];
             s_l[warp][r] = sum;
           }
-          float4* to = reinterpret_cast<float4*>(s_o + ((long)warp * rows + r) * D + g * 16);
+          float4* to = reinterpret_cast<float4*>(mine + r * D + g * 16);
 #pragma unroll
           for (int k = 0; k < 4; ++k)
             to[k] = make_float4(o[nt][2 * k][c] * unit, o[nt][2 * k][c + 2] * unit, o[nt][2 * k + 1][c] * unit,
                                 o[nt][2 * k + 1][c + 2] * unit);
         }
       }
+    if (lane == 0) s_part[warp] = last < 0 ? -1 : (warp * kStages + last) * kStage;
     __syncthreads();
     const bool whole = u0 == 0 && u1 == at.nu;
     // the part of a pair that starts here but ends elsewhere has the worker's second place
-    float* part = a.part + ((long)(2 * worker + (u0 == 0 ? 1 : 0)) * gridDim.y + tile) * ROWS * (D + 2);
+    float* part = a.part + ((long)(2 * worker + (u0 == 0 ? 1 : 0)) * gridDim.y + tile) * ROWS * kPart;
     for (int idx = threadIdx.x; idx < rows * D; idx += kThreads) {
       const int r = idx / D, d = idx % D;
       float top = -INFINITY;
 #pragma unroll
-      for (int w = 0; w < kWarps; ++w) top = fmaxf(top, s_m[w][r]);
+      for (int w = 0; w < kWarps; ++w)
+        if (s_part[w] >= 0) top = fmaxf(top, s_m[w][r]);
       const float ref = top == -INFINITY ? 0.f : top;
       float sum = 0.f, out = 0.f;
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
-        const float f = fast_exp2(s_m[w][r] - ref);
-        sum += s_l[w][r] * f;
-        out += s_o[((long)w * rows + r) * D + d] * f;
+        if (s_part[w] >= 0) {
+          const float f = fast_exp2(s_m[w][r] - ref);
+          sum += s_l[w][r] * f;
+          out += reinterpret_cast<const float*>(s_ring + s_part[w])[r * D + d] * f;
+        }
       }
       if (whole) {
         write_row(a, row_t + (r0 + r) / a.G, at.h * a.G + (r0 + r) % a.G, d, sum == 0.f ? 0.f : out / sum);
       } else {
-        part[r * (D + 2) + d] = out;
+        part[r * kPart + d] = out;
         if (d == 0) {
-          part[r * (D + 2) + D] = top;
-          part[r * (D + 2) + D + 1] = sum;
+          part[r * kPart + D] = top;
+          part[r * kPart + D + 1] = sum;
         }
       }
     }
@@ -492,9 +545,8 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) paged_attention_ker
   }
 }
 
-// Joins the pairs that span workers: the worker in whose range such a pair ends does it.
 template <int NT>
-__global__ void __launch_bounds__(kThreads) paged_attention_join_kernel(const AttnArgs a) {
+__global__ void __launch_bounds__(kJoin) paged_attention_join_kernel(const AttnArgs a) {
   constexpr int ROWS = 8 * NT;
   const long total = (long)a.cu_units[a.R] * a.Hkv, per = (total + gridDim.x - 1) / gridDim.x;
   const int worker = blockIdx.x, tile = blockIdx.y, r0 = tile * ROWS;
@@ -511,43 +563,68 @@ __global__ void __launch_bounds__(kThreads) paged_attention_join_kernel(const At
   const int row_t = a.cu_new[i], n = a.cu_new[i + 1] - row_t;
   const int rows = min(n * a.G - r0, ROWS);
   const int first = (int)((x - p + kPairCost) / per);
-  const auto place = [&](int w) {  // the first worker may start with the pair or before it
-    return a.part + ((long)(2 * w + (w == first ? 1 : 0)) * gridDim.y + tile) * ROWS * (D + 2);
+  // a thread has four dims of a row; the loads of eight parts are in flight together
+  const int parts = worker - first + 1;
+  const auto place = [&](int w, int r) {  // the first worker may start with the pair or before it
+    return a.part + (((long)(2 * (first + w) + (w == 0 ? 1 : 0)) * gridDim.y + tile) * ROWS + r) * kPart;
   };
-  for (int idx = threadIdx.x; idx < rows * D; idx += kThreads) {
-    const int r = idx / D, d = idx % D;
-    float top = -INFINITY;
-    for (int w = first; w <= worker; ++w) top = fmaxf(top, place(w)[r * (D + 2) + D]);
-    const float ref = top == -INFINITY ? 0.f : top;
-    float sum = 0.f, out = 0.f;
-    for (int w = first; w <= worker; ++w) {
-      const float* p = place(w) + r * (D + 2);
-      const float f = fast_exp2(p[D] - ref);
-      sum += p[D + 1] * f;
-      out += p[d] * f;
+  for (int idx = threadIdx.x; idx < rows * (D / 4); idx += kJoin) {
+    const int r = idx / (D / 4), d = idx % (D / 4) * 4;
+    float top = -INFINITY, sum = 0.f, out[4] = {};
+    for (int w0 = 0; w0 < parts; w0 += 8) {
+      float4 v[8];
+      float2 ml[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        if (w0 + k < parts) {
+          const float* p = place(w0 + k, r);
+          v[k] = *reinterpret_cast<const float4*>(p + d);
+          ml[k] = *reinterpret_cast<const float2*>(p + D);
+        } else {
+          v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+          ml[k] = make_float2(-INFINITY, 0.f);
+        }
+      }
+      float now = top;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) now = fmaxf(now, ml[k].x);
+      const float ref = now == -INFINITY ? 0.f : now, old = fast_exp2(top - ref);
+      sum *= old;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) out[c] *= old;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const float f = fast_exp2(ml[k].x - ref);
+        sum = fmaf(ml[k].y, f, sum);
+        out[0] = fmaf(v[k].x, f, out[0]);
+        out[1] = fmaf(v[k].y, f, out[1]);
+        out[2] = fmaf(v[k].z, f, out[2]);
+        out[3] = fmaf(v[k].w, f, out[3]);
+      }
+      top = now;
     }
-    write_row(a, row_t + (r0 + r) / a.G, h * a.G + (r0 + r) % a.G, d, sum == 0.f ? 0.f : out / sum);
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+      write_row(a, row_t + (r0 + r) / a.G, h * a.G + (r0 + r) % a.G, d + c, sum == 0.f ? 0.f : out[c] / sum);
   }
 }
 
-template <bool FP8, int NT, int STAGES>
+template <bool FP8, int NT>
 void launch(AttnArgs a, int max_rows, const at::TensorOptions& opts, cudaStream_t stream) {
-  constexpr int ROWS = 8 * NT;
+  constexpr int ROWS = 8 * NT, smem = kWarps * kStages * kStage;
   const int tiles = (max_rows + ROWS - 1) / ROWS;
   TORCH_CHECK(tiles <= 65535, "paged_attention: too many new tokens for one request");
-  const int smem = kWarps * (STAGES * kStage + std::min(max_rows, ROWS) * D * 4);
-  C10_CUDA_CHECK(ensure_dynamic_smem((const void*)paged_attention_kernel<FP8, NT, STAGES>,
-                                     kWarps * (STAGES * kStage + ROWS * D * 4)));
-  const int workers = device_sm_count() * (NT == 1 ? 2 : 1);
-  const at::Tensor part = at::empty({2L * workers * tiles * ROWS * (D + 2)}, opts.dtype(at::kFloat));
+  C10_CUDA_CHECK(ensure_dynamic_smem((const void*)paged_attention_kernel<FP8, NT>, smem));
+  const int workers = device_sm_count() * (NT == 1 ? 3 : 2);
+  const at::Tensor part = at::empty({2L * workers * tiles * ROWS * kPart}, opts.dtype(at::kFloat));
   a.part = part.data_ptr<float>();
   const dim3 grid(workers, tiles);
-  paged_attention_kernel<FP8, NT, STAGES><<<grid, kThreads, smem, stream>>>(a);
+  paged_attention_kernel<FP8, NT><<<grid, kThreads, smem, stream>>>(a);
   C10_CUDA_KERNEL_LAUNCH_CHECK();
   // the join is launched while the first kernel runs and waits for its end itself
   cudaLaunchConfig_t config{};
   config.gridDim = grid;
-  config.blockDim = dim3(kThreads);
+  config.blockDim = dim3(kJoin);
   config.stream = stream;
   cudaLaunchAttribute early{};
   early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -559,14 +636,10 @@ void launch(AttnArgs a, int max_rows, const at::TensorOptions& opts, cudaStream_
 
 template <bool FP8>
 void launch_rows(const AttnArgs& a, int max_rows, const at::TensorOptions& opts, cudaStream_t stream) {
-  if (max_rows <= 4)
-    launch<FP8, 1, 3>(a, max_rows, opts, stream);
-  else if (max_rows <= 8)
-    launch<FP8, 1, 2>(a, max_rows, opts, stream);
-  else if (max_rows <= 16)
-    launch<FP8, 2, 4>(a, max_rows, opts, stream);
+  if (max_rows <= 8)
+    launch<FP8, 1>(a, max_rows, opts, stream);
   else
-    launch<FP8, 4, 3>(a, max_rows, opts, stream);
+    launch<FP8, 2>(a, max_rows, opts, stream);
 }
 
 }  // namespace
