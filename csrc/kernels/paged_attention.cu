@@ -83,17 +83,34 @@ struct AttnArgs {
   float* part;  // [2 * workers][tiles][8 * NT][kPart]: output, maximum, sum
 };
 
+struct Found {
+  int i, c0, c1;  // a request, its first position / Hkv and its end's
+};
 // The request whose part of the costs laid end to end holds position `x`; every thread of the CTA
-// calls it.
-__device__ __forceinline__ int find_request(const AttnArgs& a, long x) {
+// calls it. `mine` is cu_units[threadIdx.x + 1], loaded before x was known.
+__device__ __forceinline__ Found find_request(const AttnArgs& a, long x, int mine) {
+  __shared__ int s_c[2];
   int i = 0;
-  for (int base = 0; base < a.R; base += (int)blockDim.x) {
+  for (int base = 0;;) {
     const int j = base + (int)threadIdx.x;
-    const int c = __syncthreads_count(j < a.R && (long)a.cu_units[j + 1] * a.Hkv <= x);
+    const bool before = j < a.R && (long)mine * a.Hkv <= x;
+    const int c = __syncthreads_count(before);
     i += c;
-    if (c < (int)blockDim.x) break;
+    if (c < (int)blockDim.x) {
+      // the last request that ends at or before x has its end as the found one's start
+      if (before && (int)threadIdx.x == c - 1) s_c[0] = mine;
+      if ((int)threadIdx.x == c) s_c[1] = mine;
+      if (c == 0 && threadIdx.x == 0) s_c[0] = base == 0 ? 0 : a.cu_units[base];
+      break;
+    }
+    base += (int)blockDim.x;
+    mine = base + (int)threadIdx.x < a.R ? a.cu_units[base + (int)threadIdx.x + 1] : 0;
   }
-  return i;
+  __syncthreads();
+  return Found{i, s_c[0], s_c[1]};
+}
+__device__ __forceinline__ int my_units(const AttnArgs& a) {
+  return (int)threadIdx.x < a.R ? a.cu_units[threadIdx.x + 1] : 0;
 }
 
 // A CTA's range of positions, walked pair by pair.
@@ -103,15 +120,15 @@ struct Walk {
   int h, u0, u1, nu;  // units [u0, u1) of nu of a pair (i, h)
   int row_t, n, len;  // the request's first packed row, new tokens, tokens
 
-  __device__ __forceinline__ void start(const AttnArgs& a, long from, long to, int request) {
+  __device__ __forceinline__ void start(const AttnArgs& a, long from, long to, const Found& at) {
     x = from;
     x_end = to;
-    i = request;
+    i = at.i;
+    c0 = at.c0;
+    c1 = at.c1;
     enter(a);
   }
   __device__ __forceinline__ void enter(const AttnArgs& a) {
-    c0 = a.cu_units[i];
-    c1 = a.cu_units[i + 1];
     row_t = a.cu_new[i];
     n = a.cu_new[i + 1] - row_t;
     len = a.kv_len[i];
@@ -121,12 +138,14 @@ struct Walk {
     while (x < x_end) {
       while (x >= (long)c1 * a.Hkv) {
         ++i;
+        c0 = c1;
+        c1 = a.cu_units[i + 1];
         enter(a);
       }
       const int cost = c1 - c0;
-      const long in = x - (long)c0 * a.Hkv;
-      h = (int)(in / cost);
-      const int p0 = (int)(in - (long)h * cost), p1 = (int)min((long)cost, p0 + (x_end - x));
+      const uint32_t in = (uint32_t)(x - (long)c0 * a.Hkv);  // the host checked that this fits
+      h = (int)(in / (uint32_t)cost);
+      const int p0 = (int)(in - (uint32_t)h * cost), p1 = (int)min((long)cost, p0 + (x_end - x));
       x += p1 - p0;
       u0 = max(0, p0 - kPairCost);
       u1 = max(0, p1 - kPairCost);
@@ -250,26 +269,27 @@ struct Ahead {
 };
 
 template <bool FP8, int NT>
-__global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) paged_attention_kernel(const AttnArgs a) {
+__global__ void __launch_bounds__(kThreads, 3) paged_attention_kernel(const AttnArgs a) {
   constexpr int ROWS = 8 * NT;
   static_assert(ROWS * D * 4 <= kStage, "a stage holds a warp's part of the merge");
   extern __shared__ __align__(128) uint8_t s_ring[];  // [kWarps][kStages][kStage]
   __shared__ __align__(16) float s_scales[kWarps][kStages][2][2];
   __shared__ float s_m[kWarps][ROWS], s_l[kWarps][ROWS];
+  __shared__ __align__(16) uint32_t s_q[NT == 1 ? 1 : 8][32][NT * 2];  // queries, where registers are short
   __shared__ int s_part[kWarps];  // where in s_ring a warp's part of the merge is, -1: it has none
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, tg = lane & 3;
   const int worker = blockIdx.x, tile = blockIdx.y, r0 = tile * ROWS, Hq = a.Hkv * a.G;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the join may take its places; it waits for the end
 
+  const int mine = my_units(a), units = a.cu_units[a.R], real_rows = a.cu_new[a.R];
   if (tile == 0)  // rows of no request
-    for (long t = a.cu_new[a.R] + worker; t < a.T; t += gridDim.x)
+    for (long t = real_rows + worker; t < a.T; t += gridDim.x)
       for (int c = threadIdx.x; c < Hq * D / 8; c += kThreads)
         *reinterpret_cast<uint4*>(a.out + t * a.o_st + c * 8) = make_uint4(0, 0, 0, 0);
-
-  const long total = (long)a.cu_units[a.R] * a.Hkv, per = (total + gridDim.x - 1) / gridDim.x;
+  const long total = (long)units * a.Hkv, per = (total + gridDim.x - 1) / gridDim.x;
   if (per * worker >= total) return;
   Walk at;
-  at.start(a, per * worker, min(total, per * (worker + 1)), find_request(a, per * worker));
+  at.start(a, per * worker, min(total, per * (worker + 1)), find_request(a, per * worker, mine));
   Ahead ahead;
   ahead.w = at;
   ahead.ring = s_ring + warp * kStages * kStage;
@@ -337,6 +357,17 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) paged_attention_ker
         limit[nt][c] = rc >= rows ? 0 : a.causal ? len - n + (r0 + rc) / a.G + 1 : len;
       }
     }
+    if constexpr (NT > 1) {  // the same in every warp: each writes its share
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (j / 2 == warp)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            s_q[j][lane][nt * 2] = qf[nt][j][0];
+            s_q[j][lane][nt * 2 + 1] = qf[nt][j][1];
+          }
+      __syncthreads();
+    }
     const int most = at.most(a, r0, rows);
     const int least = a.causal ? len - n + r0 / a.G + 1 : len;
 
@@ -357,22 +388,39 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) paged_attention_ker
       stage ^= 1;
 
       float s[2][NT][4];
+      uint4 k[2][4];
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
-        const uint4 k0 = codes(kp + half * kHalf), k1 = codes(kp + half * kHalf + k_more),
-                    k2 = codes(kp + half * kHalf + 8 * D), k3 = codes(kp + half * kHalf + 8 * D + k_more);
+        k[half][0] = codes(kp + half * kHalf);
+        k[half][1] = codes(kp + half * kHalf + k_more);
+        k[half][2] = codes(kp + half * kHalf + 8 * D);
+        k[half][3] = codes(kp + half * kHalf + 8 * D + k_more);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
           s[half][nt][0] = s[half][nt][2] = start[nt][0];
           s[half][nt][1] = s[half][nt][3] = start[nt][1];
         }
+      }
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const uint32_t lo = biased<FP8>(word(j < 4 ? k0 : k1, j & 3)), hi = biased<FP8>(word(j < 4 ? k2 : k3, j & 3));
+      for (int j = 0; j < 8; ++j) {
+        uint32_t q[NT][2];
+        if constexpr (NT == 1) {
+          q[0][0] = qf[0][j][0];
+          q[0][1] = qf[0][j][1];
+        } else {
+          const uint4 v = *reinterpret_cast<const uint4*>(s_q[j][lane]);
+          q[0][0] = v.x;
+          q[0][1] = v.y;
+          q[NT - 1][0] = v.z;
+          q[NT - 1][1] = v.w;
+        }
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const uint32_t lo = biased<FP8>(word(k[half][j / 4], j & 3)), hi = biased<FP8>(word(k[half][2 + j / 4], j & 3));
           const uint32_t a0 = widen<FP8, false, false>(lo), a2 = widen<FP8, true, false>(lo);
           const uint32_t a1 = widen<FP8, false, false>(hi), a3 = widen<FP8, true, false>(hi);
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) mma16816(s[half][nt], a0, a1, a2, a3, qf[nt][j][0], qf[nt][j][1]);
+          for (int nt = 0; nt < NT; ++nt) mma16816(s[half][nt], a0, a1, a2, a3, q[nt][0], q[nt][1]);
         }
       }
 
@@ -545,68 +593,127 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) paged_attention_ker
   }
 }
 
+// Joins the parts of the pairs that span workers. Up to kFew parts: the worker in whose range the pair
+// ends has them all, a thread four dims of a row. More (a long context and few pairs): each of
+// the pair's workers takes every so many-th row, and its warps share the row's parts.
+template <int NT>
+struct Join {
+  static constexpr int ROWS = 8 * NT, kFew = 8, JW = kJoin / 32;
+  const AttnArgs& a;
+  long per;
+  int i, h, first, parts, rows, row_t, r0, tile;
+
+  __device__ __forceinline__ const float* part(int w, int r) const {  // the first worker may start with the pair or before
+    return a.part + (((long)(2 * (first + w) + (w == 0 ? 1 : 0)) * gridDim.y + tile) * ROWS + r) * kPart;
+  }
+  // parts w0, w0 + step, ... of row r, four dims from d on, added under a common maximum
+  template <int N>
+  __device__ __forceinline__ void add(int r, int d, int w0, int step, float& top, float& sum, float (&out)[4]) const {
+    float4 v[N];
+    float2 ml[N];
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+      ml[k] = make_float2(-INFINITY, 0.f);
+      if (w0 + k * step < parts) {
+        const float* p = part(w0 + k * step, r);
+        v[k] = *reinterpret_cast<const float4*>(p + d);
+        ml[k] = *reinterpret_cast<const float2*>(p + D);
+      }
+    }
+    float now = top;
+#pragma unroll
+    for (int k = 0; k < N; ++k) now = fmaxf(now, ml[k].x);
+    const float ref = now == -INFINITY ? 0.f : now, old = fast_exp2(top - ref);
+    sum *= old;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) out[c] *= old;
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      const float f = fast_exp2(ml[k].x - ref);
+      sum = fmaf(ml[k].y, f, sum);
+      out[0] = fmaf(v[k].x, f, out[0]);
+      out[1] = fmaf(v[k].y, f, out[1]);
+      out[2] = fmaf(v[k].z, f, out[2]);
+      out[3] = fmaf(v[k].w, f, out[3]);
+    }
+    top = now;
+  }
+  __device__ __forceinline__ void write(int r, int d, float o, float l) const {
+    write_row(a, row_t + (r0 + r) / a.G, h * a.G + (r0 + r) % a.G, d, l == 0.f ? 0.f : o / l);
+  }
+  // the pair at position x, for this worker
+  __device__ __forceinline__ void pair(const Found& at, long x, int worker) {
+    const int cost = at.c1 - at.c0;
+    i = at.i;
+    h = (int)((uint32_t)(x - (long)at.c0 * a.Hkv) / (uint32_t)cost);
+    const long begin = (long)at.c0 * a.Hkv + (long)h * cost;
+    first = (int)((begin + kPairCost) / per);
+    const int last = (int)((begin + cost - 1) / per);
+    parts = last - first + 1;
+    if (parts == 1 || worker < first || (parts <= kFew && worker != last)) return;
+    row_t = a.cu_new[i];
+    rows = min((a.cu_new[i + 1] - row_t) * a.G - r0, ROWS);
+    if (parts <= kFew) {
+      for (int idx = threadIdx.x; idx < rows * (D / 4); idx += kJoin) {
+        const int r = idx / (D / 4), d = idx % (D / 4) * 4;
+        float top = -INFINITY, sum = 0.f, out[4] = {};
+        add<kFew>(r, d, 0, 1, top, sum, out);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) write(r, d + c, out[c], sum);
+      }
+      return;
+    }
+    __shared__ __align__(16) float s_out[JW][D];
+    __shared__ float s_ml[JW][2];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    for (int r = worker - first; r < rows; r += parts) {
+      float top = -INFINITY, sum = 0.f, out[4] = {};
+      for (int w0 = warp; w0 < parts; w0 += 4 * JW) add<4>(r, lane * 4, w0, JW, top, sum, out);
+      *reinterpret_cast<float4*>(&s_out[warp][lane * 4]) = make_float4(out[0], out[1], out[2], out[3]);
+      if (lane == 0) {
+        s_ml[warp][0] = top;
+        s_ml[warp][1] = sum;
+      }
+      __syncthreads();
+      if (threadIdx.x < D) {
+        float most = -INFINITY, l = 0.f, o = 0.f;
+#pragma unroll
+        for (int w = 0; w < JW; ++w) most = fmaxf(most, s_ml[w][0]);
+        const float ref = most == -INFINITY ? 0.f : most;
+#pragma unroll
+        for (int w = 0; w < JW; ++w) {
+          const float f = fast_exp2(s_ml[w][0] - ref);
+          l += s_ml[w][1] * f;
+          o += s_out[w][threadIdx.x] * f;
+        }
+        write(r, threadIdx.x, o, l);
+      }
+      __syncthreads();
+    }
+  }
+};
+
 template <int NT>
 __global__ void __launch_bounds__(kJoin) paged_attention_join_kernel(const AttnArgs a) {
-  constexpr int ROWS = 8 * NT;
+  const int mine = my_units(a), worker = blockIdx.x;
   const long total = (long)a.cu_units[a.R] * a.Hkv, per = (total + gridDim.x - 1) / gridDim.x;
-  const int worker = blockIdx.x, tile = blockIdx.y, r0 = tile * ROWS;
   const long x = per * worker, x_end = min(total, x + per);
-  if (x >= x_end) {
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    return;
+  const bool some = x < x_end;
+  Found at{0, 0, 0}, end{0, 0, 0};
+  if (some) {  // the pairs at both ends of the range; those between are whole
+    at = find_request(a, x, mine);
+    end = find_request(a, x_end - 1, mine);
   }
-  const int i = find_request(a, x), c0 = a.cu_units[i], cost = a.cu_units[i + 1] - c0;
-  const long in = x - (long)c0 * a.Hkv;
-  const int h = (int)(in / cost), p = (int)(in - (long)h * cost);
   asm volatile("griddepcontrol.wait;" ::: "memory");  // the parts are written; in every CTA, so this grid ends last
-  if (p <= kPairCost || x + (cost - p) > x_end) return;  // starts here, or goes on in the next range
-  const int row_t = a.cu_new[i], n = a.cu_new[i + 1] - row_t;
-  const int rows = min(n * a.G - r0, ROWS);
-  const int first = (int)((x - p + kPairCost) / per);
-  // a thread has four dims of a row; the loads of eight parts are in flight together
-  const int parts = worker - first + 1;
-  const auto place = [&](int w, int r) {  // the first worker may start with the pair or before it
-    return a.part + (((long)(2 * (first + w) + (w == 0 ? 1 : 0)) * gridDim.y + tile) * ROWS + r) * kPart;
-  };
-  for (int idx = threadIdx.x; idx < rows * (D / 4); idx += kJoin) {
-    const int r = idx / (D / 4), d = idx % (D / 4) * 4;
-    float top = -INFINITY, sum = 0.f, out[4] = {};
-    for (int w0 = 0; w0 < parts; w0 += 8) {
-      float4 v[8];
-      float2 ml[8];
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        if (w0 + k < parts) {
-          const float* p = place(w0 + k, r);
-          v[k] = *reinterpret_cast<const float4*>(p + d);
-          ml[k] = *reinterpret_cast<const float2*>(p + D);
-        } else {
-          v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-          ml[k] = make_float2(-INFINITY, 0.f);
-        }
-      }
-      float now = top;
-#pragma unroll
-      for (int k = 0; k < 8; ++k) now = fmaxf(now, ml[k].x);
-      const float ref = now == -INFINITY ? 0.f : now, old = fast_exp2(top - ref);
-      sum *= old;
-#pragma unroll
-      for (int c = 0; c < 4; ++c) out[c] *= old;
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const float f = fast_exp2(ml[k].x - ref);
-        sum = fmaf(ml[k].y, f, sum);
-        out[0] = fmaf(v[k].x, f, out[0]);
-        out[1] = fmaf(v[k].y, f, out[1]);
-        out[2] = fmaf(v[k].z, f, out[2]);
-        out[3] = fmaf(v[k].w, f, out[3]);
-      }
-      top = now;
-    }
-#pragma unroll
-    for (int c = 0; c < 4; ++c)
-      write_row(a, row_t + (r0 + r) / a.G, h * a.G + (r0 + r) % a.G, d + c, sum == 0.f ? 0.f : out[c] / sum);
-  }
+  if (!some) return;
+  Join<NT> join{a, per};
+  join.tile = blockIdx.y;
+  join.r0 = blockIdx.y * Join<NT>::ROWS;
+  join.pair(at, x, worker);
+  const int cost = at.c1 - at.c0;
+  const long in = x - (long)at.c0 * a.Hkv;
+  if (in / cost != (x_end - 1 - (long)at.c0 * a.Hkv) / cost || end.i != at.i) join.pair(end, x_end - 1, worker);
 }
 
 template <bool FP8, int NT>
@@ -615,7 +722,7 @@ void launch(AttnArgs a, int max_rows, const at::TensorOptions& opts, cudaStream_
   const int tiles = (max_rows + ROWS - 1) / ROWS;
   TORCH_CHECK(tiles <= 65535, "paged_attention: too many new tokens for one request");
   C10_CUDA_CHECK(ensure_dynamic_smem((const void*)paged_attention_kernel<FP8, NT>, smem));
-  const int workers = device_sm_count() * (NT == 1 ? 3 : 2);
+  const int workers = device_sm_count() * 3;
   const at::Tensor part = at::empty({2L * workers * tiles * ROWS * kPart}, opts.dtype(at::kFloat));
   a.part = part.data_ptr<float>();
   const dim3 grid(workers, tiles);
@@ -709,6 +816,7 @@ at::Tensor paged_attention(const at::Tensor& query, const at::Tensor& keys, cons
   a.o_st = out.stride(0);
   const int64_t max_rows = std::min<int64_t>(max_new, T) * a.G;
   TORCH_CHECK(max_rows < (1LL << 30), "paged_attention: too many rows");
+  TORCH_CHECK((tables.size(1) * s / kUnitKeys + kPairCost + 1) * H < (1LL << 31), "paged_attention: tables too wide");
   cudaStream_t stream = at::cuda::getCurrentCUDAStream();
   if (keys.scalar_type() == at::kFloat8_e4m3fn)
     launch_rows<true>(a, (int)std::max<int64_t>(max_rows, 1), query.options(), stream);

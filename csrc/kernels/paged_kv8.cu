@@ -15,9 +15,9 @@
 // that its new owner has not written yet contribute exact zeros when they are masked.
 // Scales of non-zero tokens are at least 2^-100: 1/S' is finite, and ratios of two scales are.
 //
-// One CTA of 128 threads takes one (run, head, key or value): 16 lanes hold a row of 128 values as
-// 16-byte loads, the run stays in registers between the maximum and the rounding, so tokens are
-// read once and codes written once.
+// One CTA takes the keys and the values of one (run, head): 16 lanes hold a row of 128
+// values as 16-byte loads, the run stays in registers between the maximum and the rounding, so
+// tokens are read once and codes written once.
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <cuda_fp8.h>
@@ -29,8 +29,6 @@ namespace hrm {
 namespace {
 
 constexpr int D = 128;
-constexpr int kThreads = 128;
-constexpr int kRowsAtOnce = kThreads / 16;
 
 template <bool FP8>
 struct Code {
@@ -90,102 +88,127 @@ struct AppendArgs {
   int H, size, T, num_blocks;
 };
 
-template <bool FP8, int ROWS>  // ROWS: rows of a run that a thread holds, size / 8
-__global__ void __launch_bounds__(kThreads) paged_append_kernel(const AppendArgs a) {
-  if ((int)blockIdx.x >= a.num_runs[0]) return;
+template <bool FP8, int THREADS, int ROWS>  // ROWS: rows of a run that a thread holds, size * 16 / THREADS
+__global__ void __launch_bounds__(THREADS) paged_append_kernel(const AppendArgs a) {
+  constexpr int kRowsAtOnce = THREADS / 16, kWarps = THREADS / 32;
   const int4 run = a.runs[blockIdx.x];  // block, first offset, tokens, first row
-  const int h = blockIdx.y, which = blockIdx.z;
+  if ((int)blockIdx.x >= a.num_runs[0]) return;
+  const int h = blockIdx.y;
   const int lane = threadIdx.x & 15, row0 = threadIdx.x >> 4;
   // a plan of another cache or another number of rows: nothing outside the tensors is touched
   if (run.x < 0 || run.x >= a.num_blocks || run.w < 0 || run.w + run.z > a.T || run.y + run.z > a.size) return;
 
-  const __nv_bfloat16* x = a.x[which] + run.w * a.x_st[which] + h * a.x_sh[which] + lane * 8;
-  uint4 held[ROWS];
-  uint32_t top = 0;  // bf16 magnitudes order as integers; at least 0x7f80 is not finite
+  const long bh = (long)run.x * a.H + h;
+  uint4 held[2][ROWS];
+  float before[2];
 #pragma unroll
-  for (int i = 0; i < ROWS; ++i) {
-    const int r = row0 + i * kRowsAtOnce;
-    held[i] = r < run.z ? *reinterpret_cast<const uint4*>(x + r * a.x_st[which]) : make_uint4(0, 0, 0, 0);
-    const uint32_t m = __vmaxu2(__vmaxu2(held[i].x & 0x7fff7fffu, held[i].y & 0x7fff7fffu),
-                                __vmaxu2(held[i].z & 0x7fff7fffu, held[i].w & 0x7fff7fffu));
-    top = __vmaxu2(top, m);
-  }
-  top = max(top & 0xffffu, top >> 16);
+  for (int c = 0; c < 2; ++c) {
+    const long st = c ? a.x_st[1] : a.x_st[0];
+    const __nv_bfloat16* x = (c ? a.x[1] : a.x[0]) + run.w * st + h * (c ? a.x_sh[1] : a.x_sh[0]) + lane * 8;
 #pragma unroll
-  for (int off = 16; off > 0; off >>= 1) top = max(top, __shfl_xor_sync(~0u, top, off));
-  __shared__ uint32_t s_top[kThreads / 32];
-  float* scale = a.scales[which] + (long)run.x * a.H + h;
-  const float before = run.y > 0 ? *scale : 0.f;
-  if ((threadIdx.x & 31) == 0) s_top[threadIdx.x >> 5] = top;
-  __syncthreads();  // also: every thread has read the scale
-  top = max(max(s_top[0], s_top[1]), max(s_top[2], s_top[3]));
-
-  const bool finite = top < 0x7f80u && before == before;
-  float now = __uint_as_float(top << 16) * (1.f / Code<FP8>::kMax);
-  if (top > 0) now = fmaxf(now, 0x1p-100f);
-  now = finite ? fmaxf(now, before) : __int_as_float(0x7fc00000);
-  const float inv = now > 0.f ? __frcp_rn(now) : 0.f;
-  uint8_t* codes = a.codes[which] + ((long)run.x * a.H + h) * a.size * D + lane * 8;
-  if (threadIdx.x == 0) *scale = now;
-
-  if (finite && before > 0.f && now != before) {  // the block's older tokens, to the wider range
-    const float ratio = before * inv;
-    for (int r = row0; r < run.y; r += kRowsAtOnce) {
-      uint2* p = reinterpret_cast<uint2*>(codes + r * D);
-      float v[8];
-      from_codes<FP8>(*p, v);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] *= ratio;
-      *p = to_codes<FP8>(v);
+    for (int i = 0; i < ROWS; ++i) {
+      const int r = row0 + i * kRowsAtOnce;
+      held[c][i] = r < run.z ? *reinterpret_cast<const uint4*>(x + r * st) : make_uint4(0, 0, 0, 0);
     }
+    before[c] = run.y > 0 ? (c ? a.scales[1] : a.scales[0])[bh] : 0.f;
   }
+  __shared__ uint32_t s_top[2][kWarps];
 #pragma unroll
-  for (int i = 0; i < ROWS; ++i) {
-    const int r = row0 + i * kRowsAtOnce;
-    if (r < run.z) {
-      uint2 out = make_uint2(0, 0);
-      if (finite) {
+  for (int c = 0; c < 2; ++c) {
+    uint32_t top = 0;  // bf16 magnitudes order as integers; at least 0x7f80 is not finite
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) {
+      const uint4 v = held[c][i];
+      top = __vmaxu2(top, __vmaxu2(__vmaxu2(v.x & 0x7fff7fffu, v.y & 0x7fff7fffu),
+                                   __vmaxu2(v.z & 0x7fff7fffu, v.w & 0x7fff7fffu)));
+    }
+    top = max(top & 0xffffu, top >> 16);
+    top = __reduce_max_sync(~0u, top);
+    if ((threadIdx.x & 31) == 0) s_top[c][threadIdx.x >> 5] = top;
+  }
+  __syncthreads();  // also: every thread has read the scales
+#pragma unroll
+  for (int c = 0; c < 2; ++c) {
+    uint32_t top = s_top[c][0];
+#pragma unroll
+    for (int w = 1; w < kWarps; ++w) top = max(top, s_top[c][w]);
+    const bool finite = top < 0x7f80u && before[c] == before[c];
+    float now = __uint_as_float(top << 16) * (1.f / Code<FP8>::kMax);
+    if (top > 0) now = fmaxf(now, 0x1p-100f);
+    now = finite ? fmaxf(now, before[c]) : __int_as_float(0x7fc00000);
+    const float inv = now > 0.f ? __frcp_rn(now) : 0.f;
+    uint8_t* codes = (c ? a.codes[1] : a.codes[0]) + bh * a.size * D + lane * 8;
+    if (threadIdx.x == 0) (c ? a.scales[1] : a.scales[0])[bh] = now;
+
+    if (finite && before[c] > 0.f && now != before[c]) {  // the block's older tokens, to the wider range
+      const float ratio = before[c] * inv;
+      for (int r = row0; r < run.y; r += kRowsAtOnce) {
+        uint2* p = reinterpret_cast<uint2*>(codes + r * D);
         float v[8];
-        unpack8(held[i], v);
+        from_codes<FP8>(*p, v);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] *= inv;
-        out = to_codes<FP8>(v);
+        for (int i = 0; i < 8; ++i) v[i] *= ratio;
+        *p = to_codes<FP8>(v);
       }
-      *reinterpret_cast<uint2*>(codes + (run.y + r) * D) = out;
+    }
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) {
+      const int r = row0 + i * kRowsAtOnce;
+      if (r < run.z) {
+        uint2 out = make_uint2(0, 0);
+        if (finite) {
+          float v[8];
+          unpack8(held[c][i], v);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) v[j] *= inv;
+          out = to_codes<FP8>(v);
+        }
+        *reinterpret_cast<uint2*>(codes + (run.y + r) * D) = out;
+      }
     }
   }
 }
 
-// Tokens back as bf16: 16 threads a (slot, head), keys and values; slot -1 (or one outside the
-// cache) gives zeros.
+// Tokens back as bf16: 16 threads a slot and kReadHeads heads, keys and values; slot -1 (or one outside
+// the cache) gives zeros.
+constexpr int kReadHeads = 4;
 template <bool FP8>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(128)
     paged_read_kernel(const uint8_t* __restrict__ kc, const uint8_t* __restrict__ vc, const float* __restrict__ ks,
-                      const float* __restrict__ vs, const int* __restrict__ slots, long items, int H, int size_log2,
+                      const float* __restrict__ vs, const int* __restrict__ slots, int N, int H, int size_log2,
                       int num_blocks, __nv_bfloat16* __restrict__ keys, __nv_bfloat16* __restrict__ values) {
-  const int lane = threadIdx.x & 15;
-  for (long it = ((long)blockIdx.x * blockDim.x + threadIdx.x) >> 4; it < items;
-       it += ((long)gridDim.x * blockDim.x) >> 4) {
-    const long n = it / H;
-    const int h = (int)(it % H), slot = slots[n];
-    uint4 out[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
-    if (slot >= 0 && (slot >> size_log2) < num_blocks) {
-      const long bh = (long)(slot >> size_log2) * H + h;
+  const int lane = threadIdx.x & 15, n = blockIdx.x * 8 + (threadIdx.x >> 4), h0 = blockIdx.y * kReadHeads;
+  if (n >= N) return;
+  const int slot = slots[n], block = slot >> size_log2;
+  const bool held = slot >= 0 && block < num_blocks;
+  uint2 w[kReadHeads][2];
+  float s[kReadHeads][2];
+#pragma unroll
+  for (int i = 0; i < kReadHeads; ++i) {
+    w[i][0] = w[i][1] = make_uint2(0, 0);
+    s[i][0] = s[i][1] = 0.f;
+    if (held && h0 + i < H) {
+      const long bh = (long)block * H + h0 + i;
       const long at = ((bh << size_log2) + (slot & ((1 << size_log2) - 1))) * D + lane * 8;
-      const uint2 w[2] = {*reinterpret_cast<const uint2*>(kc + at), *reinterpret_cast<const uint2*>(vc + at)};
-      const float s[2] = {ks[bh], vs[bh]};
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        float v[8];
-        from_codes<FP8>(w[c], v);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] *= s[c];
-        out[c] = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]),
-                            pack_bf16x2(v[6], v[7]));
-      }
+      w[i][0] = *reinterpret_cast<const uint2*>(kc + at);
+      w[i][1] = *reinterpret_cast<const uint2*>(vc + at);
+      s[i][0] = ks[bh];
+      s[i][1] = vs[bh];
     }
-    reinterpret_cast<uint4*>(keys)[it * 16 + lane] = out[0];
-    reinterpret_cast<uint4*>(values)[it * 16 + lane] = out[1];
+  }
+#pragma unroll
+  for (int i = 0; i < kReadHeads; ++i) {
+    if (h0 + i >= H) break;
+    const long to = ((long)n * H + h0 + i) * 16 + lane;
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      float v[8];
+      from_codes<FP8>(w[i][c], v);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] *= s[i][c];
+      reinterpret_cast<uint4*>(c ? values : keys)[to] = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]),
+                                                                  pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
+    }
   }
 }
 
@@ -210,11 +233,12 @@ bool check_cache(const at::Tensor& keys, const at::Tensor& values, const at::Ten
 
 template <bool FP8>
 void launch_append(const AppendArgs& a, dim3 grid, cudaStream_t stream) {
+  // 4 to 8 rows a thread: enough loads in flight, and registers for several CTAs an SM
   switch (a.size) {
-    case 16: return paged_append_kernel<FP8, 2><<<grid, kThreads, 0, stream>>>(a);
-    case 32: return paged_append_kernel<FP8, 4><<<grid, kThreads, 0, stream>>>(a);
-    case 64: return paged_append_kernel<FP8, 8><<<grid, kThreads, 0, stream>>>(a);
-    default: return paged_append_kernel<FP8, 16><<<grid, kThreads, 0, stream>>>(a);
+    case 16: return paged_append_kernel<FP8, 128, 2><<<grid, 128, 0, stream>>>(a);
+    case 32: return paged_append_kernel<FP8, 128, 4><<<grid, 128, 0, stream>>>(a);
+    case 64: return paged_append_kernel<FP8, 256, 4><<<grid, 256, 0, stream>>>(a);
+    default: return paged_append_kernel<FP8, 256, 8><<<grid, 256, 0, stream>>>(a);
   }
 }
 
@@ -257,7 +281,7 @@ void paged_append(const at::Tensor& key, const at::Tensor& value, const at::Tens
   a.size = (int)keys.size(2);
   a.T = (int)T;
   a.num_blocks = (int)keys.size(0);
-  const dim3 grid((unsigned)runs.size(0), (unsigned)H, 2);
+  const dim3 grid((unsigned)runs.size(0), (unsigned)H);
   cudaStream_t stream = at::cuda::getCurrentCUDAStream();
   if (fp8)
     launch_append<true>(a, grid, stream);
@@ -279,16 +303,16 @@ std::tuple<at::Tensor, at::Tensor> paged_read(const at::Tensor& keys, const at::
   c10::cuda::CUDAGuard guard(keys.device());
   int size_log2 = 4;
   while ((1 << size_log2) < keys.size(2)) ++size_log2;
-  const long items = N * H;
-  const int grid = (int)std::min<long>((items * 16 + 255) / 256, 1 << 20);
+  TORCH_CHECK(N < (1LL << 31) - 8 && H <= 65535LL * kReadHeads, "paged_read: too many slots or heads");
+  const dim3 grid((unsigned)((N + 7) / 8), (unsigned)((H + kReadHeads - 1) / kReadHeads));
   const auto* kc = reinterpret_cast<const uint8_t*>(keys.data_ptr());
   const auto* vc = reinterpret_cast<const uint8_t*>(values.data_ptr());
   auto* ok = reinterpret_cast<__nv_bfloat16*>(out_keys.data_ptr());
   auto* ov = reinterpret_cast<__nv_bfloat16*>(out_values.data_ptr());
   cudaStream_t stream = at::cuda::getCurrentCUDAStream();
   auto* kernel = fp8 ? paged_read_kernel<true> : paged_read_kernel<false>;
-  kernel<<<grid, 256, 0, stream>>>(kc, vc, key_scales.data_ptr<float>(), value_scales.data_ptr<float>(),
-                                   slots.data_ptr<int>(), items, (int)H, size_log2, (int)keys.size(0), ok, ov);
+  kernel<<<grid, 128, 0, stream>>>(kc, vc, key_scales.data_ptr<float>(), value_scales.data_ptr<float>(),
+                                   slots.data_ptr<int>(), (int)N, (int)H, size_log2, (int)keys.size(0), ok, ov);
   C10_CUDA_KERNEL_LAUNCH_CHECK();
   return {out_keys, out_values};
 }
