@@ -32,7 +32,8 @@ class SimpleEngine(BaseEngine):
         self.ckpt = inference_load_checkpoint(ckpt_path, ckpt_epoch, ckpt_use_ema)
 
     def generate(self, prompts: list[str], batch_size: int = 100, max_context: int = 1024,
-                 max_tokens: Optional[int] = None, temperature: float = 0.0, condition: str = "direct") -> list[str]:
+                 max_tokens: Optional[int] = None, temperature: float = 0.0, condition: str = "direct",
+                 kv_cache: str = "bf16") -> list[str]:
         from hrm_text_b200.inference.engine import inference_generate
         max_tokens = max_context if max_tokens is None else max_tokens
         outputs = [""] * len(prompts)
@@ -42,7 +43,8 @@ class SimpleEngine(BaseEngine):
             bar = tqdm(total=len(prompts), desc="generation")
         except Exception:
             bar = None
-        for pid, text in inference_generate(self.ckpt, work, max_context, max_tokens, batch_size, temperature):
+        for pid, text in inference_generate(self.ckpt, work, max_context, max_tokens, batch_size, temperature,
+                                            kv_cache=kv_cache):
             outputs[pid] = text
             if bar is not None:
                 bar.update()

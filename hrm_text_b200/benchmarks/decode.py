@@ -2,13 +2,14 @@
 ``batch`` sequences with ``context`` cached tokens each, HRM-Text L or XL, bf16, 1 GPU.
 
     python -m hrm_text_b200.benchmarks.decode [--size L|XL] [--batch 32] [--context 512]
-        [--steps 50] [--impl ours|reference]
+        [--steps 50] [--impl ours|reference] [--kv-cache bf16|int8|fp8]
 
 Both arms build the model with random-init weights, fill every slot's KV caches with random
 keys / values up to ``context`` tokens (decode cost does not depend on the values) and time
 ``steps`` decode steps with CUDA events after warm-up; the cache lengths advance by one per
 step as in generation. ``ours`` replays the CUDA graph that ``generate_tokens`` uses
-(``inference.engine.DecodeGraph``: fused kernels, no library GEMM). ``reference`` calls the
+(``inference.engine.DecodeGraph``: fused kernels, no library GEMM); with ``--kv-cache int8`` or ``fp8`` that of
+the paged 8-bit cache (``PagedDecodeGraph``, blocks assigned inside the graph). ``reference`` calls the
 reference's own ``_batched_decode`` (``torch.compile(dynamic=False, fullgraph=True)``,
 simple_inference_engine.py:110-112) on the reference model, with its KV-cache attention
 (``flash_attn_with_kvcache``) served by the FlashAttention-2 stand-in for FA3.
@@ -65,6 +66,46 @@ def run_ours(args) -> dict:
         lengths = torch.full((args.batch,), args.context, dtype=torch.int32, device=dev)
         ms = _timed(lambda: graph(tokens, lengths), args.steps, args.warmup, lengths)
     return {"impl": "ours", "ms_per_step": ms}
+
+
+def run_paged(args) -> dict:
+    from ..inference.engine import KV_CACHES, PagedDecodeGraph
+    from ..ops.paged import BlockTables
+    from ..runtime.factory import arch_preset, build_model
+    dev = torch.device("cuda", 0)
+    cfg = arch_preset("hrm", args.size) | dict(vocab_size=VOCAB, max_seq_len=MAX_SEQ_LEN)
+    torch.manual_seed(0)
+    model = build_model(cfg, dev).to(torch.bfloat16).eval()
+    width = -(-(args.context + args.steps + args.warmup + 8) // args.block_size)
+    with torch.inference_mode():
+        tables = BlockTables(args.batch * width, args.block_size, args.batch, width, dev)
+        cache = model.create_cache(paged=tables, dtype=KV_CACHES[args.kv_cache], device=dev)
+        graph = PagedDecodeGraph(model, None, cache, tables)
+        for leaf in torch.utils._pytree.tree_leaves(cache):  # random codes (bytes below e4m3's NaN), scales of values near 1
+            if leaf.dtype == torch.float32:
+                leaf.fill_(0.02)
+            else:
+                leaf.view(torch.uint8).random_(0, 120)
+        full = torch.full_like(tables.lengths, args.context)
+        tables.step(full, args.batch * args.context)
+        tokens = torch.randint(0, VOCAB, (args.batch,), device=dev)
+        active = torch.ones_like(tables.lengths)
+
+        def step():
+            graph(tokens, active)
+
+        for _ in range(args.warmup):
+            step()
+        tables.truncate(full)
+        torch.cuda.synchronize()
+        e0, e1 = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        e0.record()
+        for _ in range(args.steps):
+            step()
+        e1.record()
+        torch.cuda.synchronize()
+        tables.check()
+    return {"impl": "ours", "ms_per_step": e0.elapsed_time(e1) / args.steps}
 
 
 def _import_with_py313_generator(name: str):
@@ -127,9 +168,14 @@ def main(argv=None):
     ap.add_argument("--steps", type=int, default=50)
     ap.add_argument("--warmup", type=int, default=5)
     ap.add_argument("--impl", default="ours", choices=["ours", "reference"])
+    ap.add_argument("--kv-cache", default="bf16", choices=["bf16", "int8", "fp8"])
+    ap.add_argument("--block-size", type=int, default=64)
     args = ap.parse_args(argv)
-    out = run_ours(args) if args.impl == "ours" else run_reference(args)
-    out.update(size=args.size, batch=args.batch, context=args.context, steps=args.steps)
+    if args.impl == "reference":
+        out = run_reference(args)
+    else:
+        out = run_ours(args) if args.kv_cache == "bf16" else run_paged(args)
+    out.update(size=args.size, batch=args.batch, context=args.context, steps=args.steps, kv_cache=args.kv_cache)
     if "ms_per_step" in out:
         out["decode_tokens_per_s"] = args.batch / (out["ms_per_step"] / 1000.0)
     print(json.dumps(out))

@@ -216,7 +216,7 @@ class Attention(nn.Module):
 
     def forward(self, hidden_states: Tensor, cos_sin=None, cache: Optional[Cache] = None,
                 cache_lengths=None, prefix_lens: Optional[Tensor] = None,
-                cu_seqlens: Optional[Tensor] = None, **unused) -> Tensor:
+                cu_seqlens: Optional[Tensor] = None, prompt: bool = False, **unused) -> Tensor:
         gate, query, key, value = self.split_gqkv(self.gqkv_proj(hidden_states))
         if cos_sin is not None:
             query = apply_rotary_pos_emb(query, cos_sin)
@@ -224,6 +224,10 @@ class Attention(nn.Module):
         is_causal = self.attn_type == "causal"
         if cache is None:
             attn = prefixlm_attention_reference(query, key, value, is_causal, prefix_lens, cu_seqlens)
+        elif not isinstance(cache, Cache):  # paged: cache_lengths is the step's plan
+            from .paged import paged_cached_attention
+            return self.o_proj(paged_cached_attention(gate, query, key, value, cache, cache_lengths, is_causal,
+                                                      prompt).flatten(-2))
         else:
             attn = cached_attention(query, key, value, cache, cache_lengths, is_causal)
         gated = torch.sigmoid(gate.float()).to(attn.dtype) * attn

@@ -2,7 +2,7 @@
 
 The oracle of ``ops.paged`` and ``ops.logprobs``, and what the models run on the CPU: loops over
 requests and blocks, fp32 arithmetic in the kernels' order where the result is a code or an id
-(so those agree exactly). ``paged_kv_append`` and ``paged_kv_attention`` pick the kernels for CUDA caches.
+(so those agree exactly). ``paged_cached_attention`` is the models' attention over a paged cache.
 """
 from __future__ import annotations
 
@@ -151,9 +151,24 @@ def token_logprobs_reference(logits: Tensor, tokens: Tensor, top_k: int = 0, ign
     return lp, entropy, top, logp.gather(1, top)
 
 
-def paged_kv_append(key: Tensor, value: Tensor, cache: PagedKV8, plan: StepPlan) -> None:
-    (paged_append if cache.keys.is_cuda else paged_append_reference)(key, value, cache, plan)
+def paged_cached_attention(gate: Tensor, query: Tensor, key: Tensor, value: Tensor, cache: PagedKV8, plan: StepPlan,
+                           is_causal: bool, prompt: bool) -> Tensor:
+    """``sigmoid(gate) * attention`` of a step's packed rows (``[..., heads, 128]`` with as many rows as the plan).
 
-
-def paged_kv_attention(query: Tensor, cache: PagedKV8, plan: StepPlan, causal: bool, gate: Tensor) -> Tensor:
-    return (paged_attention if cache.keys.is_cuda else paged_attention_reference)(query, cache, plan, causal, gate)
+    The step's keys and values go into the cache. A ``prompt`` (one request's tokens into an empty cache) attends to its own
+    keys and values as they are, bidirectionally unless the layer is causal; any other step's tokens attend to the
+    cache up to themselves.
+    """
+    from .layers import prefixlm_attention_reference
+    shape = query.shape
+    gate, query, key, value = (t.reshape(-1, *t.shape[-2:]) for t in (gate, query, key, value))
+    append = paged_append if cache.keys.is_cuda else paged_append_reference
+    append(key, value, cache, plan)
+    if prompt:
+        n = query.shape[0]
+        cu, prefix = torch.tensor([0, n]), torch.tensor([n])
+        out = torch.sigmoid(gate.float()).to(query.dtype) * prefixlm_attention_reference(query, key, value, is_causal, prefix, cu)
+    else:
+        attend = paged_attention if cache.keys.is_cuda else paged_attention_reference
+        out = attend(query, cache, plan, True, gate)
+    return out.view(shape)

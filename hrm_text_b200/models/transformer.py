@@ -122,7 +122,12 @@ class Transformer(nn.Module):
             self.rotary_emb = RotaryEmbedding(config.head_dim, config.max_seq_len, base=config.rope_theta)
         self.layers = nn.ModuleList([TransformerBlock(config) for _ in range(config.n_layers)])
 
-    def create_cache(self, **kwargs) -> list[Cache]:
+    def create_cache(self, paged=None, **kwargs) -> list:
+        """One cache per layer: static bf16 ``Cache``, or ``PagedKV8`` over the blocks of ``paged`` (``BlockTables``)."""
+        if paged is not None:
+            from ..ops.paged import PagedKV8
+            return [PagedKV8.create(paged.free.numel(), paged.block_size, self.config.num_heads,
+                                    head_dim=self.config.head_dim, **kwargs) for _ in range(self.config.n_layers)]
         return [Cache.create(**kwargs, num_heads=self.config.num_heads, head_dim=self.config.head_dim)
                 for _ in range(self.config.n_layers)]
 
@@ -138,7 +143,7 @@ class Transformer(nn.Module):
                 return fused_block.stack_forward(self, x, injection, seq_info)
             if not torch.is_grad_enabled() and seq_info.get("position_ids") is not None:
                 out = fused_block.stack_forward_cached(self, x, injection, cache, seq_info.get("cache_lengths"),
-                                                       seq_info["position_ids"])
+                                                       seq_info["position_ids"], seq_info.get("prompt", False))
                 if out is not None:
                     return out
 

@@ -28,6 +28,7 @@ from ..parallel.fused import before_use
 from ..utils.trace import nvtx
 from . import gemm as G
 from .attention import PackedSeq, attention_bwd, attention_fwd, rope_half_tables
+from .paged import PagedKV8, paged_append, paged_attention
 
 
 def rmsnorm(x: Tensor, eps: float, injection: Tensor | None = None):
@@ -179,7 +180,7 @@ def stack_forward(stack, x: Tensor, injection: Tensor | None, seq_info: dict) ->
 
 
 def stack_forward_cached(stack, x: Tensor, injection: Tensor | None, cache: list, cache_lengths,
-                         position_ids: Tensor) -> Tensor | None:
+                         position_ids: Tensor, prompt: bool = False) -> Tensor | None:
     """Inference forward of a pre-norm ``Transformer`` stack against static KV caches, on the
     framework's kernels (reference models/layers.py:129-168 with ``flash_attn_with_kvcache``,
     simple_inference_engine.py:105-112).
@@ -198,6 +199,11 @@ def stack_forward_cached(stack, x: Tensor, injection: Tensor | None, cache: list
       same GEMMs, the prompt's keys / values copied into the caches, and the tcgen05 PrefixLM
       forward over the prompt (bidirectional; causal for a causal stack).
 
+    With paged caches (``ops.paged``; ``cache_lengths`` is the step's plan) the rows of ``x`` are the plan's packed rows:
+    new tokens of any requests, whose keys and values are quantised into their blocks and which attend to
+    the cache up to themselves; or, with ``prompt``, one prompt into an empty cache, which attends to its own
+    unrounded keys and values with the PrefixLM forward.
+
     Every launch is a device-side operation on static shapes, so a decode step can be captured
     in a CUDA graph.
     """
@@ -208,9 +214,10 @@ def stack_forward_cached(stack, x: Tensor, injection: Tensor | None, cache: list
     if ref.dim() != 3:
         return None
     B, S, hidden = ref.shape
-    decode = S == 1 and isinstance(cache_lengths, Tensor) and cache_lengths.numel() == B
-    prefill = B == 1 and isinstance(cache_lengths, int) and cache_lengths == 0
-    if not (decode or prefill):
+    paged = isinstance(cache[0], PagedKV8)
+    decode = not paged and S == 1 and isinstance(cache_lengths, Tensor) and cache_lengths.numel() == B
+    prefill = B == 1 and (prompt if paged else isinstance(cache_lengths, int) and cache_lengths == 0)
+    if not (decode or prefill or paged):
         return None
     cos, sin = rope_half_tables(stack.rotary_emb)
     causal = cfg.attn_type == "causal"
@@ -223,7 +230,7 @@ def stack_forward_cached(stack, x: Tensor, injection: Tensor | None, cache: list
     positions = position_ids.reshape(-1).to(torch.int32).contiguous()
     if decode:
         lengths = cache_lengths.to(device=x.device, dtype=torch.int32).contiguous()
-    else:
+    elif prefill:
         cu = torch.tensor([0, S], dtype=torch.int32, device=x.device)
         pl = torch.tensor([0 if causal else S], dtype=torch.int32, device=x.device)
         packed = PackedSeq(positions, cu, pl)
@@ -234,13 +241,18 @@ def stack_forward_cached(stack, x: Tensor, injection: Tensor | None, cache: list
         c = cache[i]
         xn, _, s = rmsnorm(x, cfg.norm_eps, inj if i == 0 else None)
         gqkv = G.infer_linear_rope(xn, a.gqkv_proj.weight, positions, cos, sin, hidden, 3 * hidden)
-        if decode:
-            y = cuda().decode_attention_gqkv(gqkv, H, c.keys, c.values, lengths)
-        else:
-            heads = gqkv.view(S, 4, H, 128)
+        heads = gqkv.view(T, 4, H, 128)
+        if paged:
+            paged_append(heads[:, 2], heads[:, 3], c, cache_lengths)
+        elif prefill:
             c.keys[0, :S].copy_(heads[:, 2])
             c.values[0, :S].copy_(heads[:, 3])
+        if prefill:
             _, y, _ = attention_fwd(gqkv, H, sched)
+        elif paged:
+            y = paged_attention(heads[:, 1], c, cache_lengths, gate=heads[:, 0]).view(T, hidden)
+        else:
+            y = cuda().decode_attention_gqkv(gqkv, H, c.keys, c.values, lengths)
         x1 = G.infer_linear(y, a.o_proj.weight, residual=s)
         xn2, _, _ = rmsnorm(x1, cfg.norm_eps)
         h = G.infer_swiglu(xn2, m.gate_up_proj.weight)
