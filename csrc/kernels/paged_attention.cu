@@ -84,79 +84,56 @@ struct AttnArgs {
 };
 
 struct Found {
-  int i, c0, c1;  // a request, its first position / Hkv and its end's
+  int i, c0, c1;      // a request, its first position / Hkv and its end's
+  int row_t, n, len;  // its first packed row, new tokens, tokens
 };
+// What this thread knows of request `j`, loaded before the position is known.
+__device__ __forceinline__ Found request_of(const AttnArgs& a, int j) {
+  if (j >= a.R) return Found{j, 0, 0, 0, 0, 0};
+  const int row_t = a.cu_new[j];
+  return Found{j, a.cu_units[j], a.cu_units[j + 1], row_t, a.cu_new[j + 1] - row_t, a.kv_len[j]};
+}
 // The request whose part of the costs laid end to end holds position `x`; every thread of the CTA
-// calls it. `mine` is cu_units[threadIdx.x + 1], loaded before x was known.
-__device__ __forceinline__ Found find_request(const AttnArgs& a, long x, int mine) {
-  __shared__ int s_c[2];
-  int i = 0;
-  for (int base = 0;;) {
-    const int j = base + (int)threadIdx.x;
-    const bool before = j < a.R && (long)mine * a.Hkv <= x;
-    const int c = __syncthreads_count(before);
-    i += c;
+// calls it. `mine` is request_of(threadIdx.x).
+__device__ __forceinline__ Found find_request(const AttnArgs& a, long x, Found mine) {
+  __shared__ Found s_found;
+  for (;;) {
+    const int c = __syncthreads_count(mine.i < a.R && (long)mine.c1 * a.Hkv <= x);
     if (c < (int)blockDim.x) {
-      // the last request that ends at or before x has its end as the found one's start
-      if (before && (int)threadIdx.x == c - 1) s_c[0] = mine;
-      if ((int)threadIdx.x == c) s_c[1] = mine;
-      if (c == 0 && threadIdx.x == 0) s_c[0] = base == 0 ? 0 : a.cu_units[base];
+      if ((int)threadIdx.x == c) s_found = mine;
       break;
     }
-    base += (int)blockDim.x;
-    mine = base + (int)threadIdx.x < a.R ? a.cu_units[base + (int)threadIdx.x + 1] : 0;
+    mine = request_of(a, mine.i + (int)blockDim.x);
   }
   __syncthreads();
-  return Found{i, s_c[0], s_c[1]};
-}
-__device__ __forceinline__ int my_units(const AttnArgs& a) {
-  return (int)threadIdx.x < a.R ? a.cu_units[threadIdx.x + 1] : 0;
+  return s_found;
 }
 
 // A CTA's range of positions, walked pair by pair.
 struct Walk {
   long x, x_end;
-  int i, c0, c1;      // a request, its first position / Hkv and its end's
-  int h, u0, u1, nu;  // units [u0, u1) of nu of a pair (i, h)
-  int row_t, n, len;  // the request's first packed row, new tokens, tokens
+  Found at;           // a request
+  int h, u0, u1, nu;  // units [u0, u1) of nu of a pair (at.i, h)
 
-  __device__ __forceinline__ void start(const AttnArgs& a, long from, long to, const Found& at) {
-    x = from;
-    x_end = to;
-    i = at.i;
-    c0 = at.c0;
-    c1 = at.c1;
-    enter(a);
-  }
-  __device__ __forceinline__ void enter(const AttnArgs& a) {
-    row_t = a.cu_new[i];
-    n = a.cu_new[i + 1] - row_t;
-    len = a.kv_len[i];
-  }
   // The next piece of a pair with rows in tile `first_row`; false at the end.
   __device__ __forceinline__ bool next(const AttnArgs& a, int first_row) {
     while (x < x_end) {
-      while (x >= (long)c1 * a.Hkv) {
-        ++i;
-        c0 = c1;
-        c1 = a.cu_units[i + 1];
-        enter(a);
-      }
-      const int cost = c1 - c0;
-      const uint32_t in = (uint32_t)(x - (long)c0 * a.Hkv);  // the host checked that this fits
+      while (x >= (long)at.c1 * a.Hkv) at = request_of(a, at.i + 1);
+      const int cost = at.c1 - at.c0;
+      const uint32_t in = (uint32_t)(x - (long)at.c0 * a.Hkv);  // the host checked that this fits
       h = (int)(in / (uint32_t)cost);
       const int p0 = (int)(in - (uint32_t)h * cost), p1 = (int)min((long)cost, p0 + (x_end - x));
       x += p1 - p0;
       u0 = max(0, p0 - kPairCost);
       u1 = max(0, p1 - kPairCost);
       nu = cost - kPairCost;
-      if (u1 > u0 && n * a.G > first_row) return true;
+      if (u1 > u0 && at.n * a.G > first_row) return true;
     }
     return false;
   }
   // keys that a row of the tile can see at most
   __device__ __forceinline__ int most(const AttnArgs& a, int first_row, int rows) const {
-    return a.causal ? len - n + (first_row + rows - 1) / a.G + 1 : len;
+    return a.causal ? at.len - at.n + (first_row + rows - 1) / a.G + 1 : at.len;
   }
 };
 
@@ -210,9 +187,18 @@ __device__ __forceinline__ uint32_t word(const uint4& v, int j) {
   return j == 0 ? v.x : j == 1 ? v.y : j == 2 ? v.z : v.w;
 }
 
-__device__ __forceinline__ void write_row(const AttnArgs& a, int t, int hq, int d, float o) {
-  if (a.gate != nullptr) o *= sigmoidf_(__bfloat162float(a.gate[t * a.g_st + hq * a.g_sh + d]));
-  a.out[t * a.o_st + (long)hq * D + d] = __float2bfloat16_rn(o);
+// Four dims of a finished row: o / l, times the gate's sigmoid.
+__device__ __forceinline__ void write_row(const AttnArgs& a, int t, int hq, int d, const float (&o)[4], float l, uint2 gate) {
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  float v[4] = {o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv};
+  if (a.gate != nullptr) {
+    const float2 lo = unpack_bf16x2(gate.x), hi = unpack_bf16x2(gate.y);
+    v[0] *= sigmoidf_(lo.x);
+    v[1] *= sigmoidf_(lo.y);
+    v[2] *= sigmoidf_(hi.x);
+    v[3] *= sigmoidf_(hi.y);
+  }
+  *reinterpret_cast<uint2*>(a.out + t * a.o_st + (long)hq * D + d) = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
 }
 
 // A warp's copies ahead: the codes and scales of its keys of every unit of the CTA's range, in order,
@@ -228,7 +214,7 @@ struct Ahead {
     live = w.next(a, first_row);
     if (live) {
       u = w.u0;
-      most = w.most(a, first_row, min(w.n * a.G - first_row, tile_rows));
+      most = w.most(a, first_row, min(w.at.n * a.G - first_row, tile_rows));
       first = u - 16;
     }
   }
@@ -240,7 +226,7 @@ struct Ahead {
         // a half after the last token takes the block, and so the scales, of the half before it
         const int kb = (u + (lane >> 1)) * kUnitKeys + warp * kKeys + (lane & 1) * 16;
         block = 0;
-        if (u + (lane >> 1) < w.u1) block = a.tables[w.i * a.table_ld + (min(kb, w.len - 1) >> a.size_log2)];
+        if (u + (lane >> 1) < w.u1) block = a.tables[w.at.i * a.table_ld + (min(kb, w.at.len - 1) >> a.size_log2)];
         if (block < 0 || block >= a.num_blocks) block = 0;  // not a table of this cache
       }
       // lane's row of each four and its 16-byte piece; the pieces of a row change places so that the
@@ -281,22 +267,25 @@ __global__ void __launch_bounds__(kThreads, 3) paged_attention_kernel(const Attn
   const int worker = blockIdx.x, tile = blockIdx.y, r0 = tile * ROWS, Hq = a.Hkv * a.G;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the join may take its places; it waits for the end
 
-  const int mine = my_units(a), units = a.cu_units[a.R], real_rows = a.cu_new[a.R];
+  const Found mine = request_of(a, threadIdx.x);
+  const int units = a.cu_units[a.R], real_rows = a.cu_new[a.R];
   if (tile == 0)  // rows of no request
     for (long t = real_rows + worker; t < a.T; t += gridDim.x)
       for (int c = threadIdx.x; c < Hq * D / 8; c += kThreads)
         *reinterpret_cast<uint4*>(a.out + t * a.o_st + c * 8) = make_uint4(0, 0, 0, 0);
   const long total = (long)units * a.Hkv, per = (total + gridDim.x - 1) / gridDim.x;
   if (per * worker >= total) return;
-  Walk at;
-  at.start(a, per * worker, min(total, per * (worker + 1)), find_request(a, per * worker, mine));
+  Walk walk;
+  walk.x = per * worker;
+  walk.x_end = min(total, walk.x + per);
+  walk.at = find_request(a, walk.x, mine);
   Ahead ahead;
-  ahead.w = at;
+  ahead.w = walk;
   ahead.ring = s_ring + warp * kStages * kStage;
   ahead.scales = s_scales[warp][0][0];
   ahead.segment(a, r0, ROWS);
-  ahead.copy(a, 0, warp, lane, r0, ROWS);
   int stage = 0;
+  bool begun = false;
   // this lane's pieces: rows g and g + 8 of the keys, pieces tg and tg + 4; rows 2 tg, 2 tg + 1 and those 8
   // below of the values, piece g
   const uint8_t* k_lane = ahead.ring + g * D + ((tg ^ ((g & 1) * 4)) << 4);
@@ -304,26 +293,28 @@ __global__ void __launch_bounds__(kThreads, 3) paged_attention_kernel(const Attn
   const uint8_t* v_lane = ahead.ring + kHalf / 2 + 2 * tg * D + ((g ^ (2 * tg)) << 4);
   const auto codes = [](const uint8_t* p) { return *reinterpret_cast<const uint4*>(p); };
 
-  while (at.next(a, r0)) {
-    const int row_t = at.row_t, n = at.n, len = at.len, u0 = at.u0, u1 = at.u1;
+  while (walk.next(a, r0)) {
+    const int row_t = walk.at.row_t, n = walk.at.n, len = walk.at.len, u0 = walk.u0, u1 = walk.u1, h = walk.h;
     const int rows = min(n * a.G - r0, ROWS);
 
     // queries as the B operand, scaled to f16; limits and logit factors of this lane's columns
+    uint4 raws[NT][4];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int rr = r0 + nt * 8 + g;
+      const __nv_bfloat16* p = a.q + (row_t + rr / a.G) * a.q_st + (h * a.G + rr % a.G) * a.q_sh + tg * 16;
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+        raws[nt][c] = rr < n * a.G ? *reinterpret_cast<const uint4*>(p + (c >> 1) * 64 + (c & 1) * 8) : make_uint4(0, 0, 0, 0);
+    }
+    if (!begun) ahead.copy(a, 0, warp, lane, r0, ROWS);  // the first codes, while the queries are on their way
+    begun = true;
     uint32_t qf[NT][8][2];
     float factor[NT][2], start[NT][2];
     int limit[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      const int r = nt * 8 + g;
-      uint4 raw[4] = {};
-      if (r < rows) {
-        const int rr = r0 + r;
-        const __nv_bfloat16* p = a.q + (row_t + rr / a.G) * a.q_st + (at.h * a.G + rr % a.G) * a.q_sh + tg * 16;
-        raw[0] = *reinterpret_cast<const uint4*>(p);
-        raw[1] = *reinterpret_cast<const uint4*>(p + 8);
-        raw[2] = *reinterpret_cast<const uint4*>(p + 64);
-        raw[3] = *reinterpret_cast<const uint4*>(p + 72);
-      }
+      const uint4(&raw)[4] = raws[nt];
       uint32_t top = 0;
 #pragma unroll
       for (int c = 0; c < 4; ++c)
@@ -368,7 +359,7 @@ __global__ void __launch_bounds__(kThreads, 3) paged_attention_kernel(const Attn
           }
       __syncthreads();
     }
-    const int most = at.most(a, r0, rows);
+    const int most = walk.most(a, r0, rows);
     const int least = a.causal ? len - n + r0 / a.G + 1 : len;
 
     float o[NT][8][4] = {}, m[NT][2] = {}, l[NT][2] = {};
@@ -560,33 +551,41 @@ __global__ void __launch_bounds__(kThreads, 3) paged_attention_kernel(const Attn
       }
     if (lane == 0) s_part[warp] = last < 0 ? -1 : (warp * kStages + last) * kStage;
     __syncthreads();
-    const bool whole = u0 == 0 && u1 == at.nu;
+    const bool whole = u0 == 0 && u1 == walk.nu;
     // the part of a pair that starts here but ends elsewhere has the worker's second place
     float* part = a.part + ((long)(2 * worker + (u0 == 0 ? 1 : 0)) * gridDim.y + tile) * ROWS * kPart;
-    for (int idx = threadIdx.x; idx < rows * D; idx += kThreads) {
-      const int r = idx / D, d = idx % D;
+    int from[kWarps];
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) from[w] = s_part[w];
+#pragma unroll 2
+    for (int idx = threadIdx.x; idx < rows * (D / 4); idx += kThreads) {  // a thread has four dims of a row
+      const int r = idx / (D / 4), d = idx % (D / 4) * 4;
+      const int t = row_t + (r0 + r) / a.G, hq = h * a.G + (r0 + r) % a.G;
+      uint2 gate = make_uint2(0, 0);
+      if (whole && a.gate != nullptr) gate = *reinterpret_cast<const uint2*>(a.gate + t * a.g_st + hq * a.g_sh + d);
       float top = -INFINITY;
 #pragma unroll
       for (int w = 0; w < kWarps; ++w)
-        if (s_part[w] >= 0) top = fmaxf(top, s_m[w][r]);
+        if (from[w] >= 0) top = fmaxf(top, s_m[w][r]);
       const float ref = top == -INFINITY ? 0.f : top;
-      float sum = 0.f, out = 0.f;
+      float sum = 0.f, out[4] = {};
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
-        if (s_part[w] >= 0) {
+        if (from[w] >= 0) {
           const float f = fast_exp2(s_m[w][r] - ref);
+          const float4 v = *reinterpret_cast<const float4*>(s_ring + from[w] + (r * D + d) * 4);
           sum += s_l[w][r] * f;
-          out += reinterpret_cast<const float*>(s_ring + s_part[w])[r * D + d] * f;
+          out[0] = fmaf(v.x, f, out[0]);
+          out[1] = fmaf(v.y, f, out[1]);
+          out[2] = fmaf(v.z, f, out[2]);
+          out[3] = fmaf(v.w, f, out[3]);
         }
       }
       if (whole) {
-        write_row(a, row_t + (r0 + r) / a.G, at.h * a.G + (r0 + r) % a.G, d, sum == 0.f ? 0.f : out / sum);
+        write_row(a, t, hq, d, out, sum, gate);
       } else {
-        part[r * kPart + d] = out;
-        if (d == 0) {
-          part[r * kPart + D] = top;
-          part[r * kPart + D + 1] = sum;
-        }
+        *reinterpret_cast<float4*>(part + r * kPart + d) = make_float4(out[0], out[1], out[2], out[3]);
+        if (d == 0) *reinterpret_cast<float2*>(part + r * kPart + D) = make_float2(top, sum);
       }
     }
     __syncthreads();
@@ -601,7 +600,7 @@ struct Join {
   static constexpr int ROWS = 8 * NT, kFew = 8, JW = kJoin / 32;
   const AttnArgs& a;
   long per;
-  int i, h, first, parts, rows, row_t, r0, tile;
+  int h, first, parts, rows, row_t, r0, tile;
 
   __device__ __forceinline__ const float* part(int w, int r) const {  // the first worker may start with the pair or before
     return a.part + (((long)(2 * (first + w) + (w == 0 ? 1 : 0)) * gridDim.y + tile) * ROWS + r) * kPart;
@@ -639,28 +638,29 @@ struct Join {
     }
     top = now;
   }
-  __device__ __forceinline__ void write(int r, int d, float o, float l) const {
-    write_row(a, row_t + (r0 + r) / a.G, h * a.G + (r0 + r) % a.G, d, l == 0.f ? 0.f : o / l);
+  __device__ __forceinline__ void write(int r, int d, const float (&o)[4], float l) const {
+    const int t = row_t + (r0 + r) / a.G, hq = h * a.G + (r0 + r) % a.G;
+    uint2 gate = make_uint2(0, 0);
+    if (a.gate != nullptr) gate = *reinterpret_cast<const uint2*>(a.gate + t * a.g_st + hq * a.g_sh + d);
+    write_row(a, t, hq, d, o, l, gate);
   }
   // the pair at position x, for this worker
   __device__ __forceinline__ void pair(const Found& at, long x, int worker) {
     const int cost = at.c1 - at.c0;
-    i = at.i;
     h = (int)((uint32_t)(x - (long)at.c0 * a.Hkv) / (uint32_t)cost);
     const long begin = (long)at.c0 * a.Hkv + (long)h * cost;
     first = (int)((begin + kPairCost) / per);
     const int last = (int)((begin + cost - 1) / per);
     parts = last - first + 1;
     if (parts == 1 || worker < first || (parts <= kFew && worker != last)) return;
-    row_t = a.cu_new[i];
-    rows = min((a.cu_new[i + 1] - row_t) * a.G - r0, ROWS);
+    row_t = at.row_t;
+    rows = min(at.n * a.G - r0, ROWS);
     if (parts <= kFew) {
       for (int idx = threadIdx.x; idx < rows * (D / 4); idx += kJoin) {
         const int r = idx / (D / 4), d = idx % (D / 4) * 4;
         float top = -INFINITY, sum = 0.f, out[4] = {};
         add<kFew>(r, d, 0, 1, top, sum, out);
-#pragma unroll
-        for (int c = 0; c < 4; ++c) write(r, d + c, out[c], sum);
+        write(r, d, out, sum);
       }
       return;
     }
@@ -676,18 +676,22 @@ struct Join {
         s_ml[warp][1] = sum;
       }
       __syncthreads();
-      if (threadIdx.x < D) {
-        float most = -INFINITY, l = 0.f, o = 0.f;
+      if (warp == 0) {
+        float most = -INFINITY, l = 0.f, o[4] = {};
 #pragma unroll
         for (int w = 0; w < JW; ++w) most = fmaxf(most, s_ml[w][0]);
         const float ref = most == -INFINITY ? 0.f : most;
 #pragma unroll
         for (int w = 0; w < JW; ++w) {
           const float f = fast_exp2(s_ml[w][0] - ref);
+          const float4 v = *reinterpret_cast<const float4*>(&s_out[w][lane * 4]);
           l += s_ml[w][1] * f;
-          o += s_out[w][threadIdx.x] * f;
+          o[0] = fmaf(v.x, f, o[0]);
+          o[1] = fmaf(v.y, f, o[1]);
+          o[2] = fmaf(v.z, f, o[2]);
+          o[3] = fmaf(v.w, f, o[3]);
         }
-        write(r, threadIdx.x, o, l);
+        write(r, lane * 4, o, l);
       }
       __syncthreads();
     }
@@ -696,11 +700,12 @@ struct Join {
 
 template <int NT>
 __global__ void __launch_bounds__(kJoin) paged_attention_join_kernel(const AttnArgs a) {
-  const int mine = my_units(a), worker = blockIdx.x;
+  const Found mine = request_of(a, threadIdx.x);
+  const int worker = blockIdx.x;
   const long total = (long)a.cu_units[a.R] * a.Hkv, per = (total + gridDim.x - 1) / gridDim.x;
   const long x = per * worker, x_end = min(total, x + per);
   const bool some = x < x_end;
-  Found at{0, 0, 0}, end{0, 0, 0};
+  Found at{}, end{};
   if (some) {  // the pairs at both ends of the range; those between are whole
     at = find_request(a, x, mine);
     end = find_request(a, x_end - 1, mine);

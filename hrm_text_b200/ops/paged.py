@@ -29,7 +29,7 @@ from .._native import cuda
 
 BLOCK_SIZES = (16, 32, 64, 128)
 CODE_TYPES = (torch.int8, torch.float8_e4m3fn)
-UNIT_KEYS, PAIR_COST = 128, 2  # how attention work is counted (csrc/kernels/paged.h)
+UNIT_KEYS, PAIR_COST = 128, 3  # how attention work is counted (csrc/kernels/paged.h)
 MAX_REQUESTS = 8192
 
 STATUS = {1: "the pool has too few free blocks", 2: "more new tokens than num_tokens", 3: "a request outgrows its table",
