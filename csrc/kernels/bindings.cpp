@@ -75,10 +75,7 @@ at::Tensor paged_attention(const at::Tensor& query, const at::Tensor& keys, cons
                            const at::Tensor& key_scales, const at::Tensor& value_scales, const at::Tensor& tables,
                            const at::Tensor& meta, int64_t max_new, bool causal, const c10::optional<at::Tensor>& gate);
 int64_t logprobs_max_top();
-std::vector<at::Tensor> token_logprobs_fwd(const at::Tensor& logits, const at::Tensor& tokens, int64_t k, bool keep);
-void token_logprobs_bwd(const at::Tensor& logits, const at::Tensor& tokens, const at::Tensor& stats,
-                        const c10::optional<at::Tensor>& g_lp, const c10::optional<at::Tensor>& g_h,
-                        const at::Tensor& grad);
+std::vector<at::Tensor> token_logprobs(const at::Tensor& logits, const at::Tensor& tokens, int64_t k);
 }  // namespace hrm
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -118,8 +115,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("paged_read", &hrm::paged_read, "keys / values of given slots back as bf16");
   m.def("paged_attention", &hrm::paged_attention, "attention of new tokens over the paged 8-bit cache, sigmoid gate fused");
   m.def("logprobs_max_top", &hrm::logprobs_max_top);
-  m.def("token_logprobs_fwd", &hrm::token_logprobs_fwd, "log probabilities of tokens, entropy and top-k of logits rows");
-  m.def("token_logprobs_bwd", &hrm::token_logprobs_bwd, "gradient of token_logprobs_fwd with respect to the logits");
+  m.def("token_logprobs", &hrm::token_logprobs,
+        "log probabilities of tokens, entropy and top-k of logits rows (differentiable)");
   m.def("device_error_word", &hrm::device_error_word);
   m.def("debug_bounds_build", &hrm::debug_bounds_build, "built with HRM_DEBUG_BOUNDS (device bounds checks)");
 }

@@ -430,20 +430,25 @@ void check_logits(const at::Tensor& logits, const at::Tensor& tokens) {
 
 int64_t logprobs_max_top() { return kGroups; }
 
-// Returns logprob and entropy [N] fp32, top_ids int64 and top_lp fp32 [N, k], and with `keep` the
-// statistics [N, 3] fp32 that the gradient needs (else an empty tensor).
+// Returns logprob and entropy [N] fp32; for k > 0 top_ids int64 and top_lp fp32 [N, k]; with `keep` last the
+// statistics [N, 3] fp32 that the gradient needs.
 std::vector<at::Tensor> token_logprobs_fwd(const at::Tensor& logits, const at::Tensor& tokens, int64_t k, bool keep) {
   check_logits(logits, tokens);
   const int64_t N = logits.size(0), V = logits.size(1);
   TORCH_CHECK(k >= 0 && k <= kGroups && k <= V, "token_logprobs: top_k is 0 to ", kGroups, " and at most the vocabulary");
   c10::cuda::CUDAGuard guard(logits.device());
   const auto f32 = logits.options().dtype(at::kFloat);
-  const at::Tensor logprob = at::empty({N}, f32), entropy = at::empty({N}, f32), top_lp = at::empty({N, k}, f32),
-                   top_ids = at::empty({N, k}, tokens.options()), stats = at::empty({keep ? N : 0, 3}, f32);
-  const std::vector<at::Tensor> out = {logprob, entropy, top_ids, top_lp, stats};
+  std::vector<at::Tensor> out = {at::empty({N}, f32), at::empty({N}, f32)};
+  if (k > 0) {
+    out.push_back(at::empty({N, k}, tokens.options()));
+    out.push_back(at::empty({N, k}, f32));
+  }
+  if (keep) out.push_back(at::empty({N, 3}, f32));
   if (N == 0) return out;
   cudaStream_t stream = at::cuda::getCurrentCUDAStream();
-  float* st = keep ? stats.data_ptr<float>() : nullptr;
+  float* st = keep ? out.back().data_ptr<float>() : nullptr;
+  int64_t* ids = k > 0 ? out[2].data_ptr<int64_t>() : nullptr;
+  float* lps = k > 0 ? out[3].data_ptr<float>() : nullptr;
   const auto run = [&](auto* x) {
     using T = std::remove_pointer_t<decltype(x)>;
     const bool few = few_rows(N);
@@ -452,8 +457,7 @@ std::vector<at::Tensor> token_logprobs_fwd(const at::Tensor& logits, const at::T
     const int64_t batches = V * (int64_t)sizeof(T) / 64 + 2 * (few ? 1024 : 128);
     const int noted = k > 1 ? (int)std::min<int64_t>(batches, kNoted) * 4 : 0;
     kernel<<<(unsigned)N, few ? 1024 : 128, noted, stream>>>(x, logits.stride(0), (int)V, tokens.data_ptr<int64_t>(), (int)k,
-                                                         logprob.data_ptr<float>(), entropy.data_ptr<float>(), st,
-                                                         top_ids.data_ptr<int64_t>(), top_lp.data_ptr<float>());
+                                                            out[0].data_ptr<float>(), out[1].data_ptr<float>(), st, ids, lps);
   };
   if (logits.scalar_type() == at::kFloat)
     run(logits.data_ptr<float>());

@@ -290,8 +290,8 @@ std::vector<at::Tensor> paged_step(const at::Tensor& tables, const at::Tensor& l
   const int64_t R = tables.size(0);
   TORCH_CHECK(fresh.device() == tables.device() && fresh.scalar_type() == at::kInt && fresh.is_contiguous() &&
                   fresh.numel() == R,
-              "paged_step: new tokens, contiguous int32 [requests] on the tables' device");
-  TORCH_CHECK(rows >= 0 && rows < (1LL << 31) - kThreads * 1024, "paged_step: number of rows");
+              "paged_step: new_tokens contiguous int32 [", R, "] on the tables' device");
+  TORCH_CHECK(rows >= 0 && rows < (1LL << 31) - kThreads * 1024, "paged_step: num_tokens ", rows);
   c10::cuda::CUDAGuard guard(tables.device());
   const auto opts = tables.options();
   const int64_t max_runs = std::min(rows, rows / block_size + 2 * R);
@@ -335,7 +335,7 @@ void paged_truncate(const at::Tensor& tables, const at::Tensor& lengths, const a
   check_state(tables, lengths, free_stack, num_free, status, done, block_size);
   TORCH_CHECK(keep.device() == tables.device() && keep.scalar_type() == at::kInt && keep.is_contiguous() &&
                   keep.numel() == lengths.numel(),
-              "paged_truncate: lengths to keep, int32 [requests]");
+              "paged_truncate: keep contiguous int32 [", lengths.numel(), "] on the tables' device");
   c10::cuda::CUDAGuard guard(tables.device());
   const int R = (int)tables.size(0);
   C10_CUDA_CHECK(ensure_dynamic_smem((const void*)paged_truncate_kernel, kMaxRequests * 4));

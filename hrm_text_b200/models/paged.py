@@ -17,9 +17,12 @@ from ..ops.paged import PAIR_COST, UNIT_KEYS, BlockTables, PagedKV8, StepPlan, p
 QMAX = {torch.int8: 127.0, torch.float8_e4m3fn: 448.0}
 
 
-def step_reference(tables: BlockTables, new_tokens: Tensor, plan: StepPlan) -> None:
-    """``BlockTables.step`` on host tensors; fills ``plan`` in place."""
-    size, rows = tables.block_size, plan.slots.numel()
+def step_reference(tables: BlockTables, new_tokens: Tensor, rows: int, max_new: int) -> StepPlan:
+    """``BlockTables.step`` on host tensors."""
+    size, R = tables.block_size, tables.lengths.numel()
+    i32 = dict(dtype=torch.int32)
+    plan = StepPlan(tables.tables, torch.empty(rows, **i32), torch.empty(rows, **i32),
+                    torch.empty((min(rows, rows // size + 2 * R), 4), **i32), torch.empty(3 * R + 3, **i32), size, max_new)
     lengths, new = tables.lengths.tolist(), new_tokens.tolist()
     blocks = lambda n: -(-n // size)  # noqa: E731
     code, at, most = 0, -1, tables.tables.shape[1] * size
@@ -60,6 +63,7 @@ def step_reference(tables: BlockTables, new_tokens: Tensor, plan: StepPlan) -> N
         plan.runs[:len(runs)] = torch.tensor(runs, dtype=torch.int32)
     tables.lengths += torch.tensor(new, dtype=torch.int32)
     tables.num_free -= rank
+    return plan
 
 
 def truncate_reference(tables: BlockTables, keep: Tensor) -> None:

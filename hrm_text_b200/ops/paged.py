@@ -124,7 +124,7 @@ class BlockTables:
         self.free = torch.arange(num_blocks - 1, -1, -1, **i32)  # low ids are handed out first
         self.num_free = torch.full((1,), num_blocks, **i32)
         self.status = torch.zeros(2, **i32)
-        self._done = torch.zeros(1, **i32)
+        self._state = (self.tables, self.lengths, self.free, self.num_free, self.status, torch.zeros(1, **i32), block_size)
 
     @classmethod
     def restore(cls, tables: Tensor, lengths: Tensor, free: Tensor, num_free: Tensor, block_size: int) -> "BlockTables":
@@ -134,8 +134,9 @@ class BlockTables:
             mine.copy_(given.reshape(mine.shape))
         return out
 
-    def _state(self):
-        return self.tables, self.lengths, self.free, self.num_free, self.status, self._done, self.block_size
+    def _check(self, value: Tensor, name: str) -> None:
+        if value.dtype is not torch.int32 or value.shape != self.lengths.shape or not value.is_contiguous():
+            raise ValueError(f"{name} must be contiguous int32 [{self.lengths.numel()}] on the tables' device")
 
     def step(self, new_tokens: Tensor, num_tokens: int, max_new: Optional[int] = None) -> StepPlan:
         """Give every request room for ``new_tokens [R]`` more tokens (int32, on the tables' device).
@@ -144,32 +145,21 @@ class BlockTables:
         ``max_new`` bounds one request's (a decode step: 1). A step that does not fit does nothing: its plan is
         empty, and ``check`` raises.
         """
-        R, dev = self.lengths.numel(), self.tables.device
-        if new_tokens.dtype != torch.int32 or new_tokens.shape != (R,) or new_tokens.device != dev:
-            raise ValueError(f"new_tokens must be int32 [{R}] on {dev}")
+        self._check(new_tokens, "new_tokens")
         if num_tokens < 0:
-            raise ValueError("num_tokens must not be negative")
+            raise ValueError(f"num_tokens must not be negative, got {num_tokens}")
         max_new = num_tokens if max_new is None else min(int(max_new), num_tokens)
-        new_tokens = new_tokens.contiguous()
-        if dev.type == "cuda":
-            return StepPlan(self.tables, *cuda().paged_step(*self._state(), new_tokens, num_tokens, max_new),
-                            self.block_size, max_new)
+        if self.tables.is_cuda:
+            return StepPlan(self.tables, *cuda().paged_step(*self._state, new_tokens, num_tokens, max_new), self.block_size,
+                            max_new)
         from ..models.paged import step_reference
-        i32 = dict(dtype=torch.int32, device=dev)
-        plan = StepPlan(self.tables, torch.empty(num_tokens, **i32), torch.empty(num_tokens, **i32),
-                        torch.empty((min(num_tokens, num_tokens // self.block_size + 2 * R), 4), **i32),
-                        torch.empty(3 * R + 3, **i32), self.block_size, max_new)
-        step_reference(self, new_tokens, plan)
-        return plan
+        return step_reference(self, new_tokens, num_tokens, max_new)
 
     def truncate(self, keep: Tensor) -> None:
         """Cut every request to at most ``keep [R]`` tokens (int32) and free its surplus blocks."""
-        R, dev = self.lengths.numel(), self.tables.device
-        if keep.dtype != torch.int32 or keep.shape != (R,) or keep.device != dev:
-            raise ValueError(f"keep must be int32 [{R}] on {dev}")
-        keep = keep.contiguous()
-        if dev.type == "cuda":
-            cuda().paged_truncate(*self._state(), keep)
+        self._check(keep, "keep")
+        if self.tables.is_cuda:
+            cuda().paged_truncate(*self._state, keep)
         else:
             from ..models.paged import truncate_reference
             truncate_reference(self, keep)

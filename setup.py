@@ -29,7 +29,7 @@ nvcc_flags = [
 if os.environ.get("HRM_DEBUG_BOUNDS", "0") == "1":
     nvcc_flags.append("-DHRM_DEBUG_BOUNDS")
 
-cuda_sources = sorted(glob.glob(os.path.join("csrc", "kernels", "*.cu"))) + ["csrc/kernels/bindings.cpp"]
+cuda_sources = sorted(glob.glob(os.path.join("csrc", "kernels", "*.cu")) + glob.glob(os.path.join("csrc", "kernels", "*.cpp")))
 
 setup(
     name="hrm_text_b200",

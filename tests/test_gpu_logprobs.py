@@ -124,6 +124,22 @@ def test_gradient_matches_differences(cuda_device):
         torch.testing.assert_close(diff, grad[:, j], rtol=0, atol=2.0 ** -11)
 
 
+def test_gradient_once_and_through_shapes(cuda_device):
+    from hrm_text_b200.ops.logprobs import token_logprobs
+    logits, tokens = _rows(6, 64, torch.float32, cuda_device)
+    leaf = logits.view(2, 3, 64).clone().requires_grad_()
+    got = token_logprobs(leaf, tokens.view(2, 3), top_k=2)
+    assert not got.top_ids.requires_grad and not got.top_logprobs.requires_grad
+    (grad,) = torch.autograd.grad(got.logprobs.sum(), leaf, create_graph=True)
+    flat = logits.clone().requires_grad_()
+    (want,) = torch.autograd.grad(token_logprobs(flat, tokens).logprobs.sum(), flat)
+    assert torch.equal(grad.detach().view(6, 64), want)
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        grad.sum().backward()
+    with torch.no_grad():
+        assert not token_logprobs(leaf, tokens.view(2, 3)).logprobs.requires_grad
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_strides_shapes_and_streams(cuda_device, dtype):
     from hrm_text_b200.ops.logprobs import token_logprobs
