@@ -265,6 +265,7 @@ __global__ void __launch_bounds__(kThreads, 3) paged_attention_kernel(const Attn
   __shared__ int s_part[kWarps];  // where in s_ring a warp's part of the merge is, -1: it has none
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, tg = lane & 3;
   const int worker = blockIdx.x, tile = blockIdx.y, r0 = tile * ROWS, Hq = a.Hkv * a.G;
+  asm volatile("griddepcontrol.wait;" ::: "memory");               // this grid starts while the kernel before it ends
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the join may take its places; it waits for the end
 
   const Found mine = request_of(a, threadIdx.x);
@@ -731,18 +732,20 @@ void launch(AttnArgs a, int max_rows, const at::TensorOptions& opts, cudaStream_
   const at::Tensor part = at::empty({2L * workers * tiles * ROWS * kPart}, opts.dtype(at::kFloat));
   a.part = part.data_ptr<float>();
   const dim3 grid(workers, tiles);
-  paged_attention_kernel<FP8, NT><<<grid, kThreads, smem, stream>>>(a);
-  C10_CUDA_KERNEL_LAUNCH_CHECK();
-  // the join is launched while the first kernel runs and waits for its end itself
-  cudaLaunchConfig_t config{};
-  config.gridDim = grid;
-  config.blockDim = dim3(kJoin);
-  config.stream = stream;
+  // both kernels are launched while the one before them ends, and wait for its end themselves
   cudaLaunchAttribute early{};
   early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   early.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t config{};
+  config.gridDim = grid;
+  config.blockDim = dim3(kThreads);
+  config.dynamicSmemBytes = smem;
+  config.stream = stream;
   config.attrs = &early;
   config.numAttrs = 1;
+  C10_CUDA_CHECK(cudaLaunchKernelEx(&config, paged_attention_kernel<FP8, NT>, a));
+  config.blockDim = dim3(kJoin);
+  config.dynamicSmemBytes = 0;
   C10_CUDA_CHECK(cudaLaunchKernelEx(&config, paged_attention_join_kernel<NT>, a));
 }
 
