@@ -73,6 +73,28 @@ def test_masked_rows(cuda_device, dtype):
     assert got.logprobs[1] == -math.inf and got.logprobs[7].isnan() and not got.entropy[7].isnan()
 
 
+@pytest.mark.parametrize("n", [3, 700])  # many threads a row, and few
+def test_few_tokens_left_by_a_mask(cuda_device, n):
+    from hrm_text_b200.ops.logprobs import token_logprobs
+    logits, tokens = _rows(n, 9000, torch.float32, cuda_device, seed=4)
+    keep = torch.zeros_like(logits, dtype=torch.bool)
+    for i in range(n):                       # left: a few at the start, in the middle, at the end; or a run of 300
+        keep[i, [(i * 7) % 50, 20, 4000 + i, 8999]] = True
+        if i % 3 == 1:
+            keep[i, 60:360] = True
+        if i % 3 == 2:
+            keep[i] = False
+            keep[i, 63] = True
+    logits.masked_fill_(~keep, -math.inf)
+    logits[0, 20] = math.nan
+    for k in (1, 20, 64):
+        got = token_logprobs(logits, tokens, k)
+        from hrm_text_b200.models.paged import token_logprobs_reference
+        want = token_logprobs_reference(logits.double(), tokens, k)
+        assert torch.equal(got.top_ids, want[2])
+        torch.testing.assert_close(got.top_logprobs.double(), want[3], rtol=2.0 ** -20, atol=2.0 ** -15, equal_nan=True)
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("n,v", [(1, 1), (3, 5), (9, 1001), (6, 32768)])
 def test_gradient_matches_formula(cuda_device, dtype, n, v):
