@@ -38,6 +38,15 @@
 // largest value scale met: P is multiplied by (scale / unit) before it is rounded, and where that
 // leaves [2^-10, 1] the unit becomes this block's scale and O is rescaled, so that small values
 // keep their bits beside large ones.
+//
+// Measured (one B200, copy rate 6.54 TB/s): 16 requests of 4000 to 40000 tokens, 8 kv heads, 4 query
+// heads each, int8: 99 us for 632 MB (98 % of the copy rate); 100 requests of 1 to 4096 tokens, 12 heads,
+// e4m3: 104 us for 663 MB (98 %). Small calls are bound by dependent loads and launches: one
+// request of 777 tokens 6.7 us, 33 requests around 600 tokens 16.8 us for 46 MB, of which about 5 us
+// pass before the first codes arrive. With 8 to 16 rows (12 requests of 300 to 6000 tokens, up to 7 new
+// ones, 2 query heads) 26 us for 96 MB: the latency of a step's chains (11 warps an SM, 46 % of the issue
+// slots used). 3 CTAs an SM (168 registers) hold 12 warps with 8 KB each in flight; 2 CTAs of 8 warps
+// with 4 KB steps were 6 and 18 % slower on the first two cases.
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <cuda_fp16.h>

@@ -292,6 +292,7 @@ class _PagedSlots:
         keep = torch.full_like(self.tables.lengths, torch.iinfo(torch.int32).max)
         keep[i] = 0
         self.tables.truncate(keep)
+        self.tables.check()  # a step that did not fit would have decoded nothing
         self.spare += self.held[i]
         self.held[i] = 0
 

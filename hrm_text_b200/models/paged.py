@@ -22,7 +22,8 @@ def step_reference(tables: BlockTables, new_tokens: Tensor, rows: int, max_new: 
     size, R = tables.block_size, tables.lengths.numel()
     i32 = dict(dtype=torch.int32)
     plan = StepPlan(tables.tables, torch.empty(rows, **i32), torch.empty(rows, **i32),
-                    torch.empty((min(rows, rows // size + 2 * R), 4), **i32), torch.empty(3 * R + 3, **i32), size, max_new)
+                    torch.empty((min(rows, rows // size + 2 * R), 4), **i32), torch.empty(3 * R + 3, **i32), size,
+                    tables.free.numel(), max_new)
     lengths, new = tables.lengths.tolist(), new_tokens.tolist()
     blocks = lambda n: -(-n // size)  # noqa: E731
     code, at, most = 0, -1, tables.tables.shape[1] * size
@@ -164,8 +165,10 @@ def paged_cached_attention(gate: Tensor, query: Tensor, key: Tensor, value: Tens
     cache up to themselves.
     """
     from .layers import prefixlm_attention_reference
-    shape = query.shape
+    shape, dtype = query.shape, query.dtype
     gate, query, key, value = (t.reshape(-1, *t.shape[-2:]) for t in (gate, query, key, value))
+    if cache.keys.is_cuda:  # the kernels' type
+        gate, query, key, value = (t.to(torch.bfloat16) for t in (gate, query, key, value))
     append = paged_append if cache.keys.is_cuda else paged_append_reference
     append(key, value, cache, plan)
     if prompt:
@@ -175,4 +178,4 @@ def paged_cached_attention(gate: Tensor, query: Tensor, key: Tensor, value: Tens
     else:
         attend = paged_attention if cache.keys.is_cuda else paged_attention_reference
         out = attend(query, cache, plan, True, gate)
-    return out.view(shape)
+    return out.view(shape).to(dtype)

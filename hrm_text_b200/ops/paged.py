@@ -83,6 +83,7 @@ class StepPlan(NamedTuple):
     runs: Tensor
     meta: Tensor  # cu_new, cu_units, kv_lengths, num_runs
     block_size: int
+    num_blocks: int
     max_new: int
 
     @property
@@ -151,7 +152,7 @@ class BlockTables:
         max_new = num_tokens if max_new is None else min(int(max_new), num_tokens)
         if self.tables.is_cuda:
             return StepPlan(self.tables, *cuda().paged_step(*self._state, new_tokens, num_tokens, max_new), self.block_size,
-                            max_new)
+                            self.free.shape[0], max_new)
         from ..models.paged import step_reference
         return step_reference(self, new_tokens, num_tokens, max_new)
 
@@ -175,8 +176,9 @@ class BlockTables:
 def _check_plan(cache: PagedKV8, plan: StepPlan, rows: int) -> None:
     if not cache.keys.is_cuda:
         raise RuntimeError("hrm_text_b200.ops.paged takes CUDA caches only (models.paged has the CPU oracle)")
-    if plan.block_size != cache.block_size:
-        raise ValueError(f"the plan is for blocks of {plan.block_size} tokens, the cache has {cache.block_size}")
+    blocks, _, size, _ = cache.keys.shape
+    if plan.block_size != size or plan.num_blocks > blocks:
+        raise ValueError(f"the plan is for {plan.num_blocks} blocks of {plan.block_size} tokens, the cache has {blocks} of {size}")
     if rows != plan.slots.numel():
         raise ValueError(f"the plan has {plan.slots.numel()} rows, got {rows}")
 

@@ -350,6 +350,8 @@ def test_refusals(cuda_device):
         paged_append(x[:2], x[:2], cache, plan)
     with pytest.raises(ValueError, match="blocks of 16"):
         paged_attention(x, PagedKV8.create(8, 32, 2, torch.int8, cuda_device), plan)
+    with pytest.raises(ValueError, match="8 blocks"):
+        paged_append(x, x, PagedKV8.create(7, 16, 2, torch.int8, cuda_device), plan)
     with pytest.raises(RuntimeError, match="bf16"):
         paged_append(x.float(), x.float(), cache, plan)
     with pytest.raises(RuntimeError, match="bf16"):
