@@ -17,8 +17,8 @@
 //
 // One CTA takes the keys and the values of one (run, head): 16 lanes hold a row of 128
 // values as 16-byte loads, the run stays in registers between the maximum and the rounding, so
-// tokens are read once and codes written once. Bound by memory for prompts: 11600 tokens of 12
-// heads, e4m3, 71 MB read and 36 MB written, 21 us (with keys and values in CTAs of their own 26 % more); by launch and load
+// tokens are read once and codes written once. Bound by memory for prompts: 14800 tokens of 12
+// heads, e4m3, 91 MB read and 45 MB written, 21 us (with keys and values in CTAs of their own 26 % more); by launch and load
 // latency for a decode step: 33 tokens of 10 heads 4.1 us.
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -172,7 +172,7 @@ __global__ void __launch_bounds__(THREADS) paged_append_kernel(const AppendArgs 
 }
 
 // Tokens back as bf16: 16 threads a slot and kReadHeads heads, keys and values; slot -1 (or one outside
-// the cache) gives zeros. 11600 tokens of 12 heads, 107 MB: 20 us (27 us with one head a thread).
+// the cache) gives zeros. 14800 tokens of 12 heads, 136 MB: 20 us (27 us with one head a thread).
 constexpr int kReadHeads = 4;
 template <bool FP8>
 __global__ void __launch_bounds__(128)
