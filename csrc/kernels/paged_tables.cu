@@ -33,6 +33,7 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
+constexpr int kRows = 4;            // rows of a step that a thread takes together
 constexpr int kMaxRequests = 8192;  // three prefix arrays of this many int32 in shared memory
 
 // status codes; the Python side names them
@@ -113,6 +114,7 @@ struct StepArgs {
 };
 
 __global__ void __launch_bounds__(kThreads) paged_step_kernel(const StepArgs a) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   extern __shared__ int sm[];
   int* s_cu = sm;              // [R + 1] first packed row of each request
   int* s_rank = s_cu + a.R + 1;  // [R] rank of its first new block
@@ -181,35 +183,58 @@ __global__ void __launch_bounds__(kThreads) paged_step_kernel(const StepArgs a) 
   }
   __syncthreads();
 
-  for (int t = blockIdx.x * kThreads + tid; t < a.rows; t += gridDim.x * kThreads) {
-    int slot = -1, pos = 0;
-    if (t < used) {
-      int lo = 0, hi = a.R;  // the last request whose first row is at or before t
-      while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (s_cu[mid] <= t)
-          lo = mid;
-        else
-          hi = mid;
-      }
-      const int i = lo, len = a.lengths[i], row = t - s_cu[i], n = s_cu[i + 1] - s_cu[i];
-      pos = len + row;
-      const int block = pos >> a.size_log2, off = pos & (size - 1), have = (int)blocks(len);
-      int id;
-      if (block < have) {
-        id = a.tables[i * a.table_ld + block];
-      } else {
-        id = a.free_stack[free_top - 1 - (s_rank[i] + block - have)];
-        if (off == 0) a.tables[i * a.table_ld + block] = id;  // a new block's first row is new
-      }
-      slot = (id << a.size_log2) + off;
-      if (row == 0 || off == 0) {
-        const int r = s_run[i] + block - (len >> a.size_log2);
-        if (r < a.max_runs) a.runs[r] = make_int4(id, off, min(size - off, n - row), t);
+  // four rows a thread: one search, and mostly one block, serves them
+  const bool wide = ((reinterpret_cast<uintptr_t>(a.slots) | reinterpret_cast<uintptr_t>(a.positions)) & 15) == 0;
+  for (int t0 = (blockIdx.x * kThreads + tid) * kRows; t0 < a.rows; t0 += gridDim.x * kThreads * kRows) {
+    int lo = 0, hi = a.R;  // the last request whose first row is at or before t0
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (s_cu[mid] <= t0)
+        lo = mid;
+      else
+        hi = mid;
+    }
+    int i = lo, len = a.lengths[i], id = -1, held_block = -1;
+    int slot[kRows], pos[kRows];
+#pragma unroll
+    for (int k = 0; k < kRows; ++k) {
+      const int t = t0 + k;
+      slot[k] = -1;
+      pos[k] = 0;
+      if (t < used) {
+        if (t >= s_cu[i + 1]) {
+          do ++i;
+          while (t >= s_cu[i + 1]);
+          len = a.lengths[i];
+          held_block = -1;
+        }
+        const int row = t - s_cu[i], n = s_cu[i + 1] - s_cu[i];
+        pos[k] = len + row;
+        const int block = pos[k] >> a.size_log2, off = pos[k] & (size - 1), have = (int)blocks(len);
+        if (block != held_block) {
+          held_block = block;
+          id = block < have ? a.tables[i * a.table_ld + block] : a.free_stack[free_top - 1 - (s_rank[i] + block - have)];
+        }
+        if (off == 0 && block >= have) a.tables[i * a.table_ld + block] = id;  // a new block's first row is new
+        slot[k] = (id << a.size_log2) + off;
+        if (row == 0 || off == 0) {
+          const int r = s_run[i] + block - (len >> a.size_log2);
+          if (r < a.max_runs) a.runs[r] = make_int4(id, off, min(size - off, n - row), t);
+        }
       }
     }
-    a.slots[t] = slot;
-    a.positions[t] = pos;
+    if (wide && t0 + kRows <= a.rows) {
+      *reinterpret_cast<int4*>(a.slots + t0) = make_int4(slot[0], slot[1], slot[2], slot[3]);
+      *reinterpret_cast<int4*>(a.positions + t0) = make_int4(pos[0], pos[1], pos[2], pos[3]);
+    } else {
+#pragma unroll
+      for (int k = 0; k < kRows; ++k) {
+        if (t0 + k < a.rows) {
+          a.slots[t0 + k] = slot[k];
+          a.positions[t0 + k] = pos[k];
+        }
+      }
+    }
   }
 
   if (last_cta(a.done)) {
@@ -228,6 +253,7 @@ __global__ void __launch_bounds__(kThreads) paged_step_kernel(const StepArgs a) 
 __global__ void __launch_bounds__(kThreads)
     paged_truncate_kernel(int* tables, long table_ld, int* lengths, const int* __restrict__ keep, int* free_stack,
                           int* num_free, int* done, int R, int size_log2) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   extern __shared__ int s_rank[];  // [R] freed blocks of the requests before
   const int size = 1 << size_log2, tid = threadIdx.x;
   const int per = (R + kThreads - 1) / kThreads, i0 = min(R, tid * per), i1 = min(R, i0 + per);
@@ -272,6 +298,22 @@ void check_state(const at::Tensor& tables, const at::Tensor& lengths, const at::
               "block tables: slots and positions are int32");
 }
 
+// Launched while the kernel before it ends; the kernels wait for that end themselves.
+template <typename... P, typename... A>
+void launch_early(void (*kernel)(P...), int grid, int smem, A... args) {
+  cudaLaunchAttribute early{};
+  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t config{};
+  config.gridDim = dim3(grid);
+  config.blockDim = dim3(kThreads);
+  config.dynamicSmemBytes = smem;
+  config.stream = at::cuda::getCurrentCUDAStream();
+  config.attrs = &early;
+  config.numAttrs = 1;
+  C10_CUDA_CHECK(cudaLaunchKernelEx(&config, kernel, args...));
+}
+
 int log2_of(int64_t v) {
   int n = 0;
   while ((int64_t(1) << n) < v) ++n;
@@ -293,7 +335,7 @@ std::vector<at::Tensor> paged_step(const at::Tensor& tables, const at::Tensor& l
   TORCH_CHECK(fresh.device() == tables.device() && fresh.scalar_type() == at::kInt && fresh.is_contiguous() &&
                   fresh.numel() == R,
               "paged_step: new_tokens contiguous int32 [", R, "] on the tables' device");
-  TORCH_CHECK(rows >= 0 && rows < (1LL << 31) - kThreads * 1024, "paged_step: num_tokens ", rows);
+  TORCH_CHECK(rows >= 0 && rows < (1LL << 31) - kThreads * 1024 * kRows, "paged_step: num_tokens ", rows);
   c10::cuda::CUDAGuard guard(tables.device());
   const auto opts = tables.options();
   const int64_t max_runs = std::min(rows, rows / block_size + 2 * R);
@@ -324,10 +366,10 @@ std::vector<at::Tensor> paged_step(const at::Tensor& tables, const at::Tensor& l
   a.num_runs = meta + 3 * R + 2;
   const int smem = (int)(3 * R + 1) * 4;
   C10_CUDA_CHECK(ensure_dynamic_smem((const void*)paged_step_kernel, (3 * kMaxRequests + 1) * 4));
-  // a CTA for each 256 rows, at most two for an SM: more would only repeat the prefix sums
-  const int64_t grid = std::max<int64_t>(1, std::min<int64_t>((rows + kThreads - 1) / kThreads, 2 * device_sm_count()));
-  paged_step_kernel<<<(int)grid, kThreads, smem, at::cuda::getCurrentCUDAStream()>>>(a);
-  C10_CUDA_KERNEL_LAUNCH_CHECK();
+  // a CTA for each 1024 rows, at most two for an SM: more would only repeat the prefix sums
+  const int64_t most = 2 * device_sm_count(), per = kThreads * kRows;
+  const int64_t grid = std::max<int64_t>(1, std::min<int64_t>((rows + per - 1) / per, most));
+  launch_early(paged_step_kernel, (int)grid, smem, a);
   return out;
 }
 
@@ -342,10 +384,9 @@ void paged_truncate(const at::Tensor& tables, const at::Tensor& lengths, const a
   const int R = (int)tables.size(0);
   C10_CUDA_CHECK(ensure_dynamic_smem((const void*)paged_truncate_kernel, kMaxRequests * 4));
   const int grid = std::max(1, std::min((R + kWarps - 1) / kWarps, 2 * device_sm_count()));
-  paged_truncate_kernel<<<grid, kThreads, R * 4, at::cuda::getCurrentCUDAStream()>>>(
-      tables.data_ptr<int>(), tables.stride(0), lengths.data_ptr<int>(), keep.data_ptr<int>(),
-      free_stack.data_ptr<int>(), num_free.data_ptr<int>(), done.data_ptr<int>(), R, log2_of(block_size));
-  C10_CUDA_KERNEL_LAUNCH_CHECK();
+  launch_early(paged_truncate_kernel, grid, R * 4, tables.data_ptr<int>(), (long)tables.stride(0), lengths.data_ptr<int>(),
+               (const int*)keep.data_ptr<int>(), free_stack.data_ptr<int>(), num_free.data_ptr<int>(), done.data_ptr<int>(), R,
+               log2_of(block_size));
 }
 
 }  // namespace hrm
