@@ -31,6 +31,7 @@
 
 #include "common.cuh"
 #include "device_setup.h"
+#include "launch_early.h"
 
 namespace hrm {
 namespace {
@@ -449,13 +450,17 @@ std::vector<at::Tensor> token_logprobs_fwd(const at::Tensor& logits, const at::T
   const int64_t N = logits.size(0), V = logits.size(1);
   TORCH_CHECK(k >= 0 && k <= kGroups && k <= V, "token_logprobs: top_k is 0 to ", kGroups, " and at most the vocabulary");
   c10::cuda::CUDAGuard guard(logits.device());
-  const auto f32 = logits.options().dtype(at::kFloat);
-  std::vector<at::Tensor> out = {at::empty({N}, f32), at::empty({N}, f32)};
+  Outputs make(logits.options());
+  make.plan({N}, at::kFloat).plan({N}, at::kFloat).plan({N, k}, at::kLong).plan({N, k}, at::kFloat);
+  std::vector<at::Tensor> out;
+  out.reserve(5);
+  out.push_back(make.next({N}, at::kFloat));
+  out.push_back(make.next({N}, at::kFloat));
   if (k > 0) {
-    out.push_back(at::empty({N, k}, tokens.options()));
-    out.push_back(at::empty({N, k}, f32));
+    out.push_back(make.next({N, k}, at::kLong));
+    out.push_back(make.next({N, k}, at::kFloat));
   }
-  if (keep) out.push_back(at::empty({N, 3}, f32));
+  if (keep) out.push_back(at::empty({N, 3}, logits.options().dtype(at::kFloat)));
   if (N == 0) return out;
   cudaStream_t stream = at::cuda::getCurrentCUDAStream();
   float* st = keep ? out.back().data_ptr<float>() : nullptr;

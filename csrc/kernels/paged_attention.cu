@@ -54,6 +54,7 @@
 
 #include "common.cuh"
 #include "device_setup.h"
+#include "launch_early.h"
 #include "paged.h"
 
 namespace hrm {
@@ -732,7 +733,7 @@ __global__ void __launch_bounds__(kJoin) paged_attention_join_kernel(const AttnA
 }
 
 template <bool FP8, int NT>
-void launch(AttnArgs a, int max_rows, const at::TensorOptions& opts, cudaStream_t stream) {
+void launch(AttnArgs a, int max_rows, const at::TensorOptions& opts) {
   constexpr int ROWS = 8 * NT, smem = kWarps * kStages * kStage;
   const int tiles = (max_rows + ROWS - 1) / ROWS;
   TORCH_CHECK(tiles <= 65535, "paged_attention: too many new tokens for one request");
@@ -741,29 +742,16 @@ void launch(AttnArgs a, int max_rows, const at::TensorOptions& opts, cudaStream_
   const at::Tensor part = at::empty({2L * workers * tiles * ROWS * kPart}, opts.dtype(at::kFloat));
   a.part = part.data_ptr<float>();
   const dim3 grid(workers, tiles);
-  // both kernels are launched while the one before them ends, and wait for its end themselves
-  cudaLaunchAttribute early{};
-  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  early.val.programmaticStreamSerializationAllowed = 1;
-  cudaLaunchConfig_t config{};
-  config.gridDim = grid;
-  config.blockDim = dim3(kThreads);
-  config.dynamicSmemBytes = smem;
-  config.stream = stream;
-  config.attrs = &early;
-  config.numAttrs = 1;
-  C10_CUDA_CHECK(cudaLaunchKernelEx(&config, paged_attention_kernel<FP8, NT>, a));
-  config.blockDim = dim3(kJoin);
-  config.dynamicSmemBytes = 0;
-  C10_CUDA_CHECK(cudaLaunchKernelEx(&config, paged_attention_join_kernel<NT>, a));
+  launch_early(paged_attention_kernel<FP8, NT>, grid, kThreads, smem, a);
+  launch_early(paged_attention_join_kernel<NT>, grid, kJoin, 0, a);
 }
 
 template <bool FP8>
-void launch_rows(const AttnArgs& a, int max_rows, const at::TensorOptions& opts, cudaStream_t stream) {
+void launch_rows(const AttnArgs& a, int max_rows, const at::TensorOptions& opts) {
   if (max_rows <= 8)
-    launch<FP8, 1>(a, max_rows, opts, stream);
+    launch<FP8, 1>(a, max_rows, opts);
   else
-    launch<FP8, 2>(a, max_rows, opts, stream);
+    launch<FP8, 2>(a, max_rows, opts);
 }
 
 }  // namespace
@@ -834,11 +822,10 @@ at::Tensor paged_attention(const at::Tensor& query, const at::Tensor& keys, cons
   const int64_t max_rows = std::min<int64_t>(max_new, T) * a.G;
   TORCH_CHECK(max_rows < (1LL << 30), "paged_attention: too many rows");
   TORCH_CHECK((tables.size(1) * s / kUnitKeys + kPairCost + 1) * H < (1LL << 31), "paged_attention: tables too wide");
-  cudaStream_t stream = at::cuda::getCurrentCUDAStream();
   if (keys.scalar_type() == at::kFloat8_e4m3fn)
-    launch_rows<true>(a, (int)std::max<int64_t>(max_rows, 1), query.options(), stream);
+    launch_rows<true>(a, (int)std::max<int64_t>(max_rows, 1), query.options());
   else
-    launch_rows<false>(a, (int)std::max<int64_t>(max_rows, 1), query.options(), stream);
+    launch_rows<false>(a, (int)std::max<int64_t>(max_rows, 1), query.options());
   return out;
 }
 

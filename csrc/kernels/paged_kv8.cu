@@ -26,6 +26,7 @@
 #include <torch/types.h>
 
 #include "common.cuh"
+#include "launch_early.h"
 
 namespace hrm {
 namespace {
@@ -93,6 +94,7 @@ struct AppendArgs {
 template <bool FP8, int THREADS, int ROWS>  // ROWS: rows of a run that a thread holds, size * 16 / THREADS
 __global__ void __launch_bounds__(THREADS) paged_append_kernel(const AppendArgs a) {
   constexpr int kRowsAtOnce = THREADS / 16, kWarps = THREADS / 32;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   const int4 run = a.runs[blockIdx.x];  // block, first offset, tokens, first row
   if ((int)blockIdx.x >= a.num_runs[0]) return;
   const int h = blockIdx.y;
@@ -179,6 +181,7 @@ __global__ void __launch_bounds__(128)
     paged_read_kernel(const uint8_t* __restrict__ kc, const uint8_t* __restrict__ vc, const float* __restrict__ ks,
                       const float* __restrict__ vs, const int* __restrict__ slots, int N, int H, int size_log2,
                       int num_blocks, __nv_bfloat16* __restrict__ keys, __nv_bfloat16* __restrict__ values) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   const int lane = threadIdx.x & 15, n = blockIdx.x * 8 + (threadIdx.x >> 4), h0 = blockIdx.y * kReadHeads;
   if (n >= N) return;
   const int slot = slots[n], block = slot >> size_log2;
@@ -234,13 +237,13 @@ bool check_cache(const at::Tensor& keys, const at::Tensor& values, const at::Ten
 }
 
 template <bool FP8>
-void launch_append(const AppendArgs& a, dim3 grid, cudaStream_t stream) {
+void launch_append(const AppendArgs& a, dim3 grid) {
   // 4 to 8 rows a thread: enough loads in flight, and registers for several CTAs an SM
   switch (a.size) {
-    case 16: return paged_append_kernel<FP8, 128, 2><<<grid, 128, 0, stream>>>(a);
-    case 32: return paged_append_kernel<FP8, 128, 4><<<grid, 128, 0, stream>>>(a);
-    case 64: return paged_append_kernel<FP8, 256, 4><<<grid, 256, 0, stream>>>(a);
-    default: return paged_append_kernel<FP8, 256, 8><<<grid, 256, 0, stream>>>(a);
+    case 16: return launch_early(paged_append_kernel<FP8, 128, 2>, grid, 128, 0, a);
+    case 32: return launch_early(paged_append_kernel<FP8, 128, 4>, grid, 128, 0, a);
+    case 64: return launch_early(paged_append_kernel<FP8, 256, 4>, grid, 256, 0, a);
+    default: return launch_early(paged_append_kernel<FP8, 256, 8>, grid, 256, 0, a);
   }
 }
 
@@ -284,12 +287,10 @@ void paged_append(const at::Tensor& key, const at::Tensor& value, const at::Tens
   a.T = (int)T;
   a.num_blocks = (int)keys.size(0);
   const dim3 grid((unsigned)runs.size(0), (unsigned)H);
-  cudaStream_t stream = at::cuda::getCurrentCUDAStream();
   if (fp8)
-    launch_append<true>(a, grid, stream);
+    launch_append<true>(a, grid);
   else
-    launch_append<false>(a, grid, stream);
-  C10_CUDA_KERNEL_LAUNCH_CHECK();
+    launch_append<false>(a, grid);
 }
 
 // slots [N] int32 -> keys, values [N, H, 128] bf16.
@@ -299,8 +300,9 @@ std::tuple<at::Tensor, at::Tensor> paged_read(const at::Tensor& keys, const at::
   const int64_t N = slots.numel(), H = keys.size(1);
   TORCH_CHECK(slots.device() == keys.device() && slots.scalar_type() == at::kInt && slots.is_contiguous(),
               "paged_read: contiguous int32 slots on the cache's device");
-  const auto opts = key_scales.options().dtype(at::kBFloat16);
-  const at::Tensor out_keys = at::empty({N, H, D}, opts), out_values = at::empty({N, H, D}, opts);
+  Outputs make(key_scales.options());
+  make.plan({N, H, D}, at::kBFloat16).plan({N, H, D}, at::kBFloat16);
+  const at::Tensor out_keys = make.next({N, H, D}, at::kBFloat16), out_values = make.next({N, H, D}, at::kBFloat16);
   if (N == 0) return {out_keys, out_values};
   c10::cuda::CUDAGuard guard(keys.device());
   int size_log2 = 4;
@@ -311,11 +313,8 @@ std::tuple<at::Tensor, at::Tensor> paged_read(const at::Tensor& keys, const at::
   const auto* vc = reinterpret_cast<const uint8_t*>(values.data_ptr());
   auto* ok = reinterpret_cast<__nv_bfloat16*>(out_keys.data_ptr());
   auto* ov = reinterpret_cast<__nv_bfloat16*>(out_values.data_ptr());
-  cudaStream_t stream = at::cuda::getCurrentCUDAStream();
-  auto* kernel = fp8 ? paged_read_kernel<true> : paged_read_kernel<false>;
-  kernel<<<grid, 128, 0, stream>>>(kc, vc, key_scales.data_ptr<float>(), value_scales.data_ptr<float>(),
-                                   slots.data_ptr<int>(), (int)N, (int)H, size_log2, (int)keys.size(0), ok, ov);
-  C10_CUDA_KERNEL_LAUNCH_CHECK();
+  launch_early(fp8 ? paged_read_kernel<true> : paged_read_kernel<false>, grid, 128, 0, kc, vc, key_scales.data_ptr<float>(),
+               value_scales.data_ptr<float>(), slots.data_ptr<int>(), (int)N, (int)H, size_log2, (int)keys.size(0), ok, ov);
   return {out_keys, out_values};
 }
 

@@ -26,6 +26,7 @@
 
 #include "common.cuh"
 #include "device_setup.h"
+#include "launch_early.h"
 #include "paged.h"
 
 namespace hrm {
@@ -298,22 +299,6 @@ void check_state(const at::Tensor& tables, const at::Tensor& lengths, const at::
               "block tables: slots and positions are int32");
 }
 
-// Launched while the kernel before it ends; the kernels wait for that end themselves.
-template <typename... P, typename... A>
-void launch_early(void (*kernel)(P...), int grid, int smem, A... args) {
-  cudaLaunchAttribute early{};
-  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  early.val.programmaticStreamSerializationAllowed = 1;
-  cudaLaunchConfig_t config{};
-  config.gridDim = dim3(grid);
-  config.blockDim = dim3(kThreads);
-  config.dynamicSmemBytes = smem;
-  config.stream = at::cuda::getCurrentCUDAStream();
-  config.attrs = &early;
-  config.numAttrs = 1;
-  C10_CUDA_CHECK(cudaLaunchKernelEx(&config, kernel, args...));
-}
-
 int log2_of(int64_t v) {
   int n = 0;
   while ((int64_t(1) << n) < v) ++n;
@@ -337,10 +322,15 @@ std::vector<at::Tensor> paged_step(const at::Tensor& tables, const at::Tensor& l
               "paged_step: new_tokens contiguous int32 [", R, "] on the tables' device");
   TORCH_CHECK(rows >= 0 && rows < (1LL << 31) - kThreads * 1024 * kRows, "paged_step: num_tokens ", rows);
   c10::cuda::CUDAGuard guard(tables.device());
-  const auto opts = tables.options();
   const int64_t max_runs = std::min(rows, rows / block_size + 2 * R);
-  std::vector<at::Tensor> out = {at::empty({rows}, opts), at::empty({rows}, opts), at::empty({max_runs, 4}, opts),
-                                 at::empty({3 * R + 3}, opts)};
+  Outputs make(tables.options());
+  make.plan({rows}, at::kInt).plan({rows}, at::kInt).plan({max_runs, 4}, at::kInt).plan({3 * R + 3}, at::kInt);
+  std::vector<at::Tensor> out;
+  out.reserve(4);
+  out.push_back(make.next({rows}, at::kInt));
+  out.push_back(make.next({rows}, at::kInt));
+  out.push_back(make.next({max_runs, 4}, at::kInt));
+  out.push_back(make.next({3 * R + 3}, at::kInt));
   int* meta = out[3].data_ptr<int>();
   StepArgs a{};
   a.tables = tables.data_ptr<int>();
@@ -369,7 +359,7 @@ std::vector<at::Tensor> paged_step(const at::Tensor& tables, const at::Tensor& l
   // a CTA for each 1024 rows, at most two for an SM: more would only repeat the prefix sums
   const int64_t most = 2 * device_sm_count(), per = kThreads * kRows;
   const int64_t grid = std::max<int64_t>(1, std::min<int64_t>((rows + per - 1) / per, most));
-  launch_early(paged_step_kernel, (int)grid, smem, a);
+  launch_early(paged_step_kernel, dim3((unsigned)grid), kThreads, smem, a);
   return out;
 }
 
@@ -384,9 +374,9 @@ void paged_truncate(const at::Tensor& tables, const at::Tensor& lengths, const a
   const int R = (int)tables.size(0);
   C10_CUDA_CHECK(ensure_dynamic_smem((const void*)paged_truncate_kernel, kMaxRequests * 4));
   const int grid = std::max(1, std::min((R + kWarps - 1) / kWarps, 2 * device_sm_count()));
-  launch_early(paged_truncate_kernel, grid, R * 4, tables.data_ptr<int>(), (long)tables.stride(0), lengths.data_ptr<int>(),
-               (const int*)keep.data_ptr<int>(), free_stack.data_ptr<int>(), num_free.data_ptr<int>(), done.data_ptr<int>(), R,
-               log2_of(block_size));
+  launch_early(paged_truncate_kernel, dim3(grid), kThreads, R * 4, tables.data_ptr<int>(), tables.stride(0),
+               lengths.data_ptr<int>(), keep.data_ptr<int>(), free_stack.data_ptr<int>(), num_free.data_ptr<int>(),
+               done.data_ptr<int>(), R, log2_of(block_size));
 }
 
 }  // namespace hrm
