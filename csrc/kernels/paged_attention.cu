@@ -738,7 +738,9 @@ void launch(AttnArgs a, int max_rows, const at::TensorOptions& opts) {
   const int tiles = (max_rows + ROWS - 1) / ROWS;
   TORCH_CHECK(tiles <= 65535, "paged_attention: too many new tokens for one request");
   C10_CUDA_CHECK(ensure_dynamic_smem((const void*)paged_attention_kernel<FP8, NT>, smem));
-  const int workers = device_sm_count() * 3;
+  // with many tiles (a request with many new tokens) fewer ranges a tile: the grid stays at about four waves,
+  // the workspace under 32 MB
+  const int resident = device_sm_count() * 3, workers = tiles <= 4 ? resident : std::max(1, 4 * resident / tiles);
   const at::Tensor part = at::empty({2L * workers * tiles * ROWS * kPart}, opts.dtype(at::kFloat));
   a.part = part.data_ptr<float>();
   const dim3 grid(workers, tiles);

@@ -223,6 +223,29 @@ def test_attention_matches_64_bits(cuda_device, dtype, heads, group, size, lengt
     assert torch.equal(out, paged_attention(q, cache, plan, causal, gt))  # the same bits again
 
 
+@pytest.mark.parametrize("chunk,group", [(700, 2), (5000, 1)])  # 88 and 313 tiles of rows
+def test_attention_many_new_tokens(cuda_device, chunk, group):
+    """A chunk of a prompt on a cached beginning, beside a decoding request; the workspace stays bounded."""
+    from hrm_text_b200.models.paged import paged_attention_reference
+    from hrm_text_b200.ops.paged import paged_append, paged_attention
+    bt, cache, _ = _filled(cuda_device, torch.int8, 2, 64, [300, 1000], extra=chunk + 64)
+    plan = bt.step(_i32([chunk, 1], cuda_device), chunk + 1)
+    bt.check()
+    x = torch.randn(chunk + 1, 2, 2, 128, device=cuda_device).bfloat16()
+    paged_append(x[:, 0], x[:, 1], cache, plan)
+    q = torch.randn(chunk + 1, 2 * group, 128, device=cuda_device).bfloat16()
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    out = paged_attention(q, cache, plan)
+    torch.cuda.synchronize()
+    assert torch.cuda.max_memory_allocated() - before < (64 << 20) + out.numel() * 2
+    rows = torch.arange(0, chunk + 1, 37, device=cuda_device)
+    rows[-1] = chunk
+    want = paged_attention_reference(q.double(), cache, plan, dtype=torch.float64)
+    _close(out[rows], want[rows], cache)
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 def test_attention_peaked_scores_and_ranges(cuda_device, dtype):
     """Scores of hundreds, blocks whose value ranges differ by 2^60, rows of tiny or huge queries."""
