@@ -17,9 +17,10 @@
 // loads a thread, in L2) instead of waiting for another kernel or CTA; the rows are spread over
 // the CTAs and find their request by binary search in shared memory. The CTA that finishes last
 // (a counter that it puts back to zero) moves lengths and num_free, after every CTA has read
-// them. These calls are bound by launch and dependent-load latency, not by bytes: a decode step of 25
-// requests 4.5 us, 512 prompts of half a million tokens 10.8 us (8 CTAs an SM instead of 2: 13.3 us, the
-// prefix sums again in each), a truncate 3.5 to 4.5 us.
+// them. These calls are bound by launch and dependent-load latency, not by bytes: a truncate and a
+// decode step of 25 requests take 8 us together, a truncate and the step of 512 prompts of half a million tokens
+// 12 us (15 us with one row a thread; 8 CTAs an SM instead of 2 were 2.5 us slower, the prefix sums again in
+// each).
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/types.h>

@@ -325,12 +325,18 @@ def test_decode_step_in_a_graph_crosses_blocks(cuda_device):
     from hrm_text_b200.ops.paged import paged_append, paged_attention
     bt, cache, _ = _filled(cuda_device, torch.int8, 2, 16, [14, 30, 1], extra=200)
     ones = _i32([1, 1, 1], cuda_device)
-    x = torch.randn(3, 4, 2, 128, device=cuda_device).bfloat16()
+    source, x = (torch.randn(3, 4, 2, 128, device=cuda_device).bfloat16() for _ in range(2))
+    queries, kept = torch.empty_like(x), torch.empty_like(x[:, 1])
 
-    def step():
+    def step():  # with copies, which are no kernels, before and after the calls
+        bt.truncate(bt.lengths.clone())
         plan = bt.step(ones, 3, max_new=1)
+        x.copy_(source)
         paged_append(x[:, 2], x[:, 3], cache, plan)
-        return plan, paged_attention(x[:, 1], cache, plan, gate=x[:, 0])
+        queries.copy_(source)
+        out = paged_attention(queries[:, 1], cache, plan, gate=queries[:, 0])
+        kept.copy_(out)
+        return plan, kept
 
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())
@@ -341,7 +347,7 @@ def test_decode_step_in_a_graph_crosses_blocks(cuda_device):
     with torch.cuda.graph(graph):
         plan, out = step()
     for _ in range(40):
-        x.copy_(torch.randn_like(x.float()))
+        source.copy_(torch.randn_like(x.float()))
         graph.replay()
         want = paged_attention_reference(x[:, 1].double(), cache, plan, gate=x[:, 0], dtype=torch.float64)
         _close(out, want, cache)
