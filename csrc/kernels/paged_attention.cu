@@ -30,9 +30,8 @@
 //   * the m index of O^T likewise: a lane owns 16 dims of four keys, pairs of keys are
 //     interleaved by byte permutes before they are widened;
 //   * P^T is S^T transposed 8x8 by movmatrix.
-// Codes are exact in f16: e4m3 by one cvt, int8 as 1152 + c by one byte permute. Values subtract the
-// 1152; for keys the accumulators start at -1152 sum q instead. Queries are scaled by a power of two
-// to a row maximum in [1, 2) before they are rounded to f16: a bf16 value keeps all its bits
+// Codes are exact in f16: e4m3 by one cvt, int8 as 1152 + c by one byte permute, less 1152. Queries are
+// scaled by a power of two to a row maximum in [1, 2) before they are rounded to f16: a bf16 value keeps all its bits
 // unless it is 2^-14 of the row's largest. P is rounded to f16 (11 bits, against 8 of bf16), sums
 // stay fp32. The key scale multiplies the fp32 score. O is held in multiples of a unit, the
 // largest value scale met: P is multiplied by (scale / unit) before it is rounded, and where that
@@ -40,9 +39,9 @@
 // keep their bits beside large ones.
 //
 // Measured (one B200, copy rate 6.54 TB/s): 16 requests of 4000 to 40000 tokens, 8 kv heads, 4 query
-// heads each, int8: 99 us for 632 MB (98 % of the copy rate); 100 requests of 1 to 4096 tokens, 12 heads,
+// heads each, int8: 100 us for 632 MB (97 % of the copy rate); 100 requests of 1 to 4096 tokens, 12 heads,
 // e4m3: 104 us for 663 MB (98 %). Small calls are bound by dependent loads and launches: one
-// request of 777 tokens 6.7 us, 33 requests around 600 tokens 16.8 us for 46 MB, of which about 5 us
+// request of 777 tokens 6.8 us, 33 requests around 600 tokens 17 us for 46 MB, of which about 5 us
 // pass before the first codes arrive. With 8 to 16 rows (12 requests of 300 to 6000 tokens, up to 7 new
 // ones, 2 query heads) 26 us for 96 MB: the latency of a step's chains (11 warps an SM, 46 % of the issue
 // slots used). 3 CTAs an SM (168 registers) hold 12 warps with 8 KB each in flight; 2 CTAs of 8 warps
@@ -157,18 +156,16 @@ __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_gr
 __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group 0;" ::: "memory"); }
 
 // Two codes, in bytes 0 and 1 (HI: 2 and 3) of a word, as f16x2: e4m3 themselves; int8, given as code + 128,
-// as 1024 + that, less 1152 for values (EXACT) and not for keys.
-template <bool FP8, bool HI, bool EXACT>
+// as 1024 + that, less 1152.
+template <bool FP8, bool HI>
 __device__ __forceinline__ uint32_t widen(uint32_t w) {
   uint32_t r;
   if constexpr (FP8) {
     asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"((unsigned short)(HI ? w >> 16 : w)));
   } else {
     r = __byte_perm(w, 0x64646464u, HI ? 0x4342 : 0x4140);
-    if constexpr (EXACT) {
-      const __half2 v = __hsub2(*reinterpret_cast<__half2*>(&r), __half2half2(__ushort_as_half(0x6480)));
-      r = *reinterpret_cast<const uint32_t*>(&v);
-    }
+    const __half2 v = __hsub2(*reinterpret_cast<__half2*>(&r), __half2half2(__ushort_as_half(0x6480)));
+    r = *reinterpret_cast<const uint32_t*>(&v);
   }
   return r;
 }
@@ -321,7 +318,7 @@ __global__ void __launch_bounds__(kThreads, 3) paged_attention_kernel(const Attn
     if (!begun) ahead.copy(a, 0, warp, lane, r0, ROWS);  // the first codes, while the queries are on their way
     begun = true;
     uint32_t qf[NT][8][2];
-    float factor[NT][2], start[NT][2];
+    float factor[NT][2];
     int limit[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
@@ -337,24 +334,18 @@ __global__ void __launch_bounds__(kThreads, 3) paged_attention_kernel(const Attn
       // 2^-e with e the exponent of the largest magnitude (within what a float can hold)
       const int e = min(126, max(-126, (int)(top >> 7) - 127));
       const float down = __uint_as_float((uint32_t)(127 - e) << 23);
-      float sum = 0.f;
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           const float2 v = unpack_bf16x2(word(raw[j / 2], (j & 1) * 2 + c));
           qf[nt][j][c] = pack_f16x2(v.x * down, v.y * down);
-          const float2 w = __half22float2(*reinterpret_cast<const __half2*>(&qf[nt][j][c]));
-          sum += w.x + w.y;
         }
       }
-      sum += __shfl_xor_sync(~0u, sum, 1);
-      sum += __shfl_xor_sync(~0u, sum, 2);
       const float up = __uint_as_float((uint32_t)(127 + e) << 23) * a.scale_log2;
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         factor[nt][c] = __shfl_sync(~0u, up, (2 * tg + c) * 4);
-        start[nt][c] = FP8 ? 0.f : -1152.f * __shfl_sync(~0u, sum, (2 * tg + c) * 4);
         const int rc = nt * 8 + 2 * tg + c;
         limit[nt][c] = rc >= rows ? 0 : a.causal ? len - n + (r0 + rc) / a.G + 1 : len;
       }
@@ -389,7 +380,7 @@ __global__ void __launch_bounds__(kThreads, 3) paged_attention_kernel(const Attn
       const uint8_t *kp = k_lane + stage * kStage, *vp = v_lane + stage * kStage;
       stage ^= 1;
 
-      float s[2][NT][4];
+      float s[2][NT][4] = {};
       uint4 k[2][4];
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
@@ -397,11 +388,6 @@ __global__ void __launch_bounds__(kThreads, 3) paged_attention_kernel(const Attn
         k[half][1] = codes(kp + half * kHalf + k_more);
         k[half][2] = codes(kp + half * kHalf + 8 * D);
         k[half][3] = codes(kp + half * kHalf + 8 * D + k_more);
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          s[half][nt][0] = s[half][nt][2] = start[nt][0];
-          s[half][nt][1] = s[half][nt][3] = start[nt][1];
-        }
       }
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
@@ -419,8 +405,8 @@ __global__ void __launch_bounds__(kThreads, 3) paged_attention_kernel(const Attn
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
           const uint32_t lo = biased<FP8>(word(k[half][j / 4], j & 3)), hi = biased<FP8>(word(k[half][2 + j / 4], j & 3));
-          const uint32_t a0 = widen<FP8, false, false>(lo), a2 = widen<FP8, true, false>(lo);
-          const uint32_t a1 = widen<FP8, false, false>(hi), a3 = widen<FP8, true, false>(hi);
+          const uint32_t a0 = widen<FP8, false>(lo), a2 = widen<FP8, true>(lo);
+          const uint32_t a1 = widen<FP8, false>(hi), a3 = widen<FP8, true>(hi);
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) mma16816(s[half][nt], a0, a1, a2, a3, q[nt][0], q[nt][1]);
         }
@@ -526,8 +512,8 @@ __global__ void __launch_bounds__(kThreads, 3) paged_attention_kernel(const Attn
 #pragma unroll
           for (int two = 0; two < 2; ++two) {  // two of the word's four dims
             const uint32_t lo = __byte_perm(w0, w1, two ? 0x7362 : 0x5140), hi = __byte_perm(w2, w3, two ? 0x7362 : 0x5140);
-            const uint32_t a0 = widen<FP8, false, true>(lo), a1 = widen<FP8, true, true>(lo);
-            const uint32_t a2 = widen<FP8, false, true>(hi), a3 = widen<FP8, true, true>(hi);
+            const uint32_t a0 = widen<FP8, false>(lo), a1 = widen<FP8, true>(lo);
+            const uint32_t a2 = widen<FP8, false>(hi), a3 = widen<FP8, true>(hi);
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) mma16816(o[nt][2 * j + two], a0, a1, a2, a3, pb[nt][0], pb[nt][1]);
           }
