@@ -59,7 +59,6 @@ void adam_atan2(const at::Tensor& p, const at::Tensor& g, const c10::optional<at
 void cast_f32_bf16(const at::Tensor& src, const at::Tensor& dst);
 at::Tensor device_error_word();
 bool debug_bounds_build();
-int64_t paged_max_requests();
 std::vector<at::Tensor> paged_step(const at::Tensor& tables, const at::Tensor& lengths, const at::Tensor& free_stack,
                                    const at::Tensor& num_free, const at::Tensor& status, const at::Tensor& done,
                                    int64_t block_size, const at::Tensor& fresh, int64_t rows, int64_t max_new);
@@ -74,7 +73,6 @@ std::tuple<at::Tensor, at::Tensor> paged_read(const at::Tensor& keys, const at::
 at::Tensor paged_attention(const at::Tensor& query, const at::Tensor& keys, const at::Tensor& values,
                            const at::Tensor& key_scales, const at::Tensor& value_scales, const at::Tensor& tables,
                            const at::Tensor& meta, int64_t max_new, bool causal, const c10::optional<at::Tensor>& gate);
-int64_t logprobs_max_top();
 std::vector<at::Tensor> token_logprobs(const at::Tensor& logits, const at::Tensor& tokens, int64_t k);
 }  // namespace hrm
 
@@ -108,13 +106,11 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("ce_dlogits", &hrm::ce_dlogits);
   m.def("adam_atan2", &hrm::adam_atan2);
   m.def("cast_f32_bf16", &hrm::cast_f32_bf16);
-  m.def("paged_max_requests", &hrm::paged_max_requests);
   m.def("paged_step", &hrm::paged_step, "assign blocks, slots and positions to the new tokens of every request");
   m.def("paged_truncate", &hrm::paged_truncate, "cut requests to given lengths and free their surplus blocks");
   m.def("paged_append", &hrm::paged_append, "quantise new keys / values into their blocks (8 bits, a scale a block and head)");
   m.def("paged_read", &hrm::paged_read, "keys / values of given slots back as bf16");
   m.def("paged_attention", &hrm::paged_attention, "attention of new tokens over the paged 8-bit cache, sigmoid gate fused");
-  m.def("logprobs_max_top", &hrm::logprobs_max_top);
   m.def("token_logprobs", &hrm::token_logprobs,
         "log probabilities of tokens, entropy and top-k of logits rows (differentiable)");
   m.def("device_error_word", &hrm::device_error_word);

@@ -441,8 +441,6 @@ void check_logits(const at::Tensor& logits, const at::Tensor& tokens) {
 
 }  // namespace
 
-int64_t logprobs_max_top() { return kGroups; }
-
 // Returns logprob and entropy [N] fp32; for k > 0 top_ids int64 and top_lp fp32 [N, k]; with `keep` last the
 // statistics [N, 3] fp32 that the gradient needs.
 std::vector<at::Tensor> token_logprobs_fwd(const at::Tensor& logits, const at::Tensor& tokens, int64_t k, bool keep) {

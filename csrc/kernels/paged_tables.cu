@@ -308,8 +308,6 @@ int log2_of(int64_t v) {
 
 }  // namespace
 
-int64_t paged_max_requests() { return kMaxRequests; }
-
 // One step: see the head of this file. Returns int32 tensors: slots and positions [rows]; runs
 // [max_runs, 4] (block, first offset, tokens, first row); meta, which is cu_new [R + 1], cu_units
 // [R + 1], kv_lengths [R] and the number of runs, one after the other.

@@ -14,7 +14,7 @@ from torch import Tensor
 
 from .._native import cuda
 
-MAX_TOP_K = 64
+MAX_TOP_K = 64  # groups of threads in the kernel
 
 
 class TokenLogprobs(NamedTuple):
