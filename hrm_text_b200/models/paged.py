@@ -150,8 +150,11 @@ def token_logprobs_reference(logits: Tensor, tokens: Tensor, top_k: int = 0, ign
     wild = ~skip & ((tokens < 0) | (tokens >= logits.shape[1]))
     lp = logp.gather(1, tokens.clamp(0, logits.shape[1] - 1)[:, None])[:, 0]
     lp = torch.where(skip, torch.zeros_like(lp), torch.where(wild, torch.full_like(lp, math.nan), lp))
+    # NaN above everything, then by value (-0 and 0 are equal), the lowest id first among equals
     order = torch.sort(torch.where(logits.isnan(), torch.full_like(logits, math.inf), logits) + 0.0, dim=-1, descending=True,
                        stable=True).indices
+    first = torch.sort(logits.isnan().gather(1, order).to(torch.int8), dim=-1, descending=True, stable=True).indices
+    order = order.gather(1, first)
     top = order[:, :top_k]
     return lp, entropy, top, logp.gather(1, top)
 
