@@ -351,14 +351,15 @@ __global__ void __launch_bounds__(THREADS)
     }
     return;
   }
-  // too many at the bound: the largest below the last one found, k times
+  // too many at the bound: the largest, then the largest below the last one found; the key of a NaN at id 0 is
+  // all ones, so nothing is below a start from there
   __syncthreads();
-  unsigned long long last = ~0ull;
+  unsigned long long last = 0;
   for (int at = 0; at < k; ++at) {
     unsigned long long mine = 0;
     for (int j = tid; j < V; j += THREADS) {
       const unsigned long long c = rank_key(value(x[j]), j);
-      if (c < last && c > mine) mine = c;
+      if ((at == 0 || c < last) && c > mine) mine = c;
     }
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) mine = max(mine, __shfl_xor_sync(~0u, mine, off));

@@ -1,0 +1,42 @@
+"""Log probabilities where the rows decide which kernel runs, and the row's first places.
+
+Rows run on 1024, 128 or 64 threads (many threads a row for few rows). Tolerances: a thread adds V / (2 threads)
+terms in each of two chains, then the chains and the threads are joined and a running maximum moves a few times, so S is
+good to r = (V / (2 threads) + 40) 2^-24 + 2^-18 (the second for the exponentials: 2^-22 each, and the rounding of
+their arguments, 2^-24 |x - m| with |x - m| < 60 where a term counts). All terms of W have one sign, so W / S is good to
+2 r |W / S| and the entropy to r (1 + 2 |log S - H|). A log probability takes two more roundings of itself.
+Gradients: p to r + 2^-17, H as above, one rounding to the logits' type.
+"""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+def _rows(n, v, dtype, device, seed=0):
+    g = torch.Generator(device=device).manual_seed(seed)
+    x = torch.randn(n, v, generator=g, device=device) * 3
+    x[:, :: max(1, v // 3)] += 8
+    return x.to(dtype), torch.randint(0, v, (n,), generator=g, device=device)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n", [6, 700])
+def test_nan_at_the_first_id(cuda_device, dtype, n):
+    """NaN is above everything, lowest id first, also where a row is too long or too even to be ranked by counting."""
+    from hrm_text_b200.models.paged import token_logprobs_reference
+    from hrm_text_b200.ops.logprobs import token_logprobs
+    logits, tokens = _rows(n, 32768, dtype, cuda_device, seed=1)
+    logits[0, 0] = math.nan
+    logits[1] = math.nan
+    logits[2, ::2] = math.nan
+    logits[3, 0], logits[3, 77] = math.inf, math.nan
+    logits[4] = 1.0                              # equal values: id 0 first
+    logits[5, 1:] = -math.inf
+    for k in (1, 5, 64):
+        got = token_logprobs(logits, tokens, k)
+        want = token_logprobs_reference(logits[:6].double(), tokens[:6], k)
+        assert torch.equal(got.top_ids[:6], want[2])
+        assert got.top_ids[0, 0] == 0 and got.top_ids[1].tolist() == list(range(k)) and got.top_ids[3, 0] == 77
