@@ -270,9 +270,9 @@ __global__ void __launch_bounds__(THREADS)
       const float h = empty ? 0.f : log_s - acc.w / acc.s;
       entropy[row] = h;
       if (stats != nullptr) {
-        stats[row * 3] = m;
-        stats[row * 3 + 1] = log_s;
-        stats[row * 3 + 2] = h;
+        stats[(long)row * 3] = m;
+        stats[(long)row * 3 + 1] = log_s;
+        stats[(long)row * 3 + 2] = h;
       }
       s_m = m;
       s_log_s = log_s;
@@ -382,7 +382,7 @@ __global__ void __launch_bounds__(THREADS)
   const T* x = logits + row * ld;
   T* out = grad + row * ldg;
   const int64_t t = tokens[row];
-  const float m = stats[row * 3], log_s = stats[row * 3 + 1], h = stats[row * 3 + 2];
+  const float m = stats[(long)row * 3], log_s = stats[(long)row * 3 + 1], h = stats[(long)row * 3 + 2];
   float glp = g_lp != nullptr && t != kIgnore ? g_lp[row] : 0.f;
   if (t != kIgnore && (t < 0 || t >= V)) glp = NAN;
   if (log_s == INFINITY) glp = 0.f;  // a row of nothing

@@ -40,3 +40,22 @@ def test_nan_at_the_first_id(cuda_device, dtype, n):
         want = token_logprobs_reference(logits[:6].double(), tokens[:6], k)
         assert torch.equal(got.top_ids[:6], want[2])
         assert got.top_ids[0, 0] == 0 and got.top_ids[1].tolist() == list(range(k)) and got.top_ids[3, 0] == 77
+
+
+def test_rows_past_32_bits_of_statistics(cuda_device):
+    """The statistics are three numbers a row: from 715,827,883 rows on their index passes 31 bits."""
+    from hrm_text_b200.ops.logprobs import token_logprobs
+    n = 715_827_883 + 40
+    leaf = torch.tensor([[0.5, 2.0]], device=cuda_device).bfloat16().requires_grad_()
+    tokens = torch.ones(n, dtype=torch.long, device=cuda_device)
+    tokens[-1] = 0
+    got = token_logprobs(leaf.expand(n, 2), tokens)
+    want = torch.log_softmax(torch.tensor([0.5, 2.0]), -1).tolist()
+    assert torch.allclose(got.logprobs[-50:-1].cpu(), torch.full((49,), want[1]), rtol=0, atol=2.0 ** -18)
+    assert abs(got.logprobs[-1].item() - want[0]) < 2.0 ** -18
+    logits = leaf.detach().expand(n, 2).requires_grad_()
+    (grad,) = torch.autograd.grad(token_logprobs(logits, tokens).logprobs.sum(), logits)
+    p = math.exp(want[1])
+    rest = torch.tensor([p - 1, 1 - p]).bfloat16().expand(49, 2)  # bf16 gradients, to one step of theirs
+    assert torch.allclose(grad[-50:-1].float().cpu(), rest.float(), rtol=2.0 ** -7, atol=0)
+    assert torch.allclose(grad[-1].float().cpu(), torch.tensor([p, -p]), rtol=2.0 ** -7, atol=0)
