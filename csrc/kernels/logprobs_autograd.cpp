@@ -48,6 +48,8 @@ struct TokenLogprobs : torch::autograd::Function<TokenLogprobs> {
 
 // logprob, entropy and for k > 0 top_ids, top_logprobs of logits [N, V]; differentiable where the logits are.
 std::vector<at::Tensor> token_logprobs(const at::Tensor& logits, const at::Tensor& tokens, int64_t k) {
+  // a dual tensor need not require a gradient, and its tangent would be lost in the kernel's outputs
+  TORCH_CHECK(!logits._fw_grad(/*level=*/0).defined(), "token_logprobs has no forward-mode derivative");
   if (at::GradMode::is_enabled() && logits.requires_grad()) return TokenLogprobs::apply(logits, tokens, k);
   return token_logprobs_fwd(logits, tokens, k, false);
 }

@@ -33,7 +33,7 @@ def token_logprobs(logits: Tensor, tokens: Tensor, top_k: int = 0) -> TokenLogpr
     ``logits [..., V]`` fp32 or bf16 (rows contiguous, any row stride), ``tokens [...]`` integer ids; a token of
     -100 (``IGNORE_LABEL_ID``) has log probability 0 and no gradient, any other id outside the vocabulary
     gives NaN. A row of minus infinities has log probability -inf, entropy 0 and no gradient. ``logprobs``
-    and ``entropy`` are differentiable (once); the top log probabilities are not.
+    and ``entropy`` are differentiable (once, backwards only); the top log probabilities are not.
     """
     if not logits.is_cuda:
         raise RuntimeError("hrm_text_b200.ops.logprobs takes CUDA tensors only (models.paged has the CPU oracle)")

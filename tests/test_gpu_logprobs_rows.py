@@ -59,3 +59,13 @@ def test_rows_past_32_bits_of_statistics(cuda_device):
     rest = torch.tensor([p - 1, 1 - p]).bfloat16().expand(49, 2)  # bf16 gradients, to one step of theirs
     assert torch.allclose(grad[-50:-1].float().cpu(), rest.float(), rtol=2.0 ** -7, atol=0)
     assert torch.allclose(grad[-1].float().cpu(), torch.tensor([p, -p]), rtol=2.0 ** -7, atol=0)
+
+
+def test_forward_gradients_are_refused(cuda_device):
+    import torch.autograd.forward_ad as fwd
+    from hrm_text_b200.ops.logprobs import token_logprobs
+    logits, tokens = _rows(2, 100, torch.float32, cuda_device)
+    for leaf in (logits, logits.clone().requires_grad_()):
+        with fwd.dual_level(), pytest.raises(RuntimeError, match="forward"):
+            token_logprobs(fwd.make_dual(leaf, torch.ones_like(leaf)), tokens)
+    token_logprobs(logits, tokens)
