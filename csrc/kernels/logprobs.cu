@@ -7,8 +7,8 @@
 // Differences x - m are taken before anything is multiplied, so a token that is alone has log p
 // exactly 0 and large logits lose nothing. Minus infinity, and anything far below m, adds exact
 // zeros; a row of minus infinities alone has log p = -inf, H = 0 and a zero gradient. A NaN or
-// plus infinity makes the row's values NaN. A token of -100 has log p = 0, any other outside the
-// vocabulary NaN.
+// plus infinity makes the row's values NaN. A token of -100 has log p = 0 and no gradient of it, any other outside
+// the vocabulary NaN for both; the row's entropy and its gradient do not depend on the token.
 //
 // The k likeliest (k <= 64, larger first, the lowest index first among equals): the threads are 64
 // groups, and k groups hold a value of at least the k-th largest of the groups' largest values, so
@@ -384,7 +384,7 @@ __global__ void __launch_bounds__(THREADS)
   const int64_t t = tokens[row];
   const float m = stats[(long)row * 3], log_s = stats[(long)row * 3 + 1], h = stats[(long)row * 3 + 2];
   float glp = g_lp != nullptr && t != kIgnore ? g_lp[row] : 0.f;
-  if (t != kIgnore && (t < 0 || t >= V)) glp = NAN;
+  if (g_lp != nullptr && t != kIgnore && (t < 0 || t >= V)) glp = NAN;  // the entropy does not depend on the token
   if (log_s == INFINITY) glp = 0.f;  // a row of nothing
   const float gh = g_h != nullptr ? g_h[row] : 0.f;
   const float a = -(glp + gh * h);

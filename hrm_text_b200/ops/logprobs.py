@@ -31,8 +31,9 @@ def token_logprobs(logits: Tensor, tokens: Tensor, top_k: int = 0) -> TokenLogpr
     """``log softmax(logits)[tokens]``, the entropy of ``softmax(logits)`` and its ``top_k`` likeliest tokens.
 
     ``logits [..., V]`` fp32 or bf16 (rows contiguous, any row stride), ``tokens [...]`` integer ids; a token of
-    -100 (``IGNORE_LABEL_ID``) has log probability 0 and no gradient, any other id outside the vocabulary
-    gives NaN. A row of minus infinities has log probability -inf, entropy 0 and no gradient. ``logprobs``
+    -100 (``IGNORE_LABEL_ID``) has log probability 0 and no gradient of it, any other id outside the vocabulary
+    gives NaN for both. A row's entropy, and the entropy's gradient, do not depend on its token: mask them
+    where a padded row must not count. A row of minus infinities has log probability -inf, entropy 0 and no gradient. ``logprobs``
     and ``entropy`` are differentiable (once, backwards only); the top log probabilities are not.
     """
     if not logits.is_cuda:

@@ -69,3 +69,27 @@ def test_forward_gradients_are_refused(cuda_device):
         with fwd.dual_level(), pytest.raises(RuntimeError, match="forward"):
             token_logprobs(fwd.make_dual(leaf, torch.ones_like(leaf)), tokens)
     token_logprobs(logits, tokens)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_gradient_of_an_id_outside_the_vocabulary(cuda_device, dtype):
+    """Its log probability is NaN and so is the gradient of it; the entropy, and the entropy's gradient, do not depend on it."""
+    from hrm_text_b200.ops.logprobs import token_logprobs
+    logits, tokens = _rows(5, 1001, dtype, cuda_device, seed=2)
+    inside = tokens.clone()
+    tokens[1], tokens[2], tokens[3] = 1001, -1, -100
+    g_lp, g_h = (torch.randn(5, device=cuda_device) for _ in range(2))
+
+    def grad(ids, use_lp, use_h):
+        leaf = logits.clone().requires_grad_()
+        got = token_logprobs(leaf, ids)
+        outs = [o for o, use in ((got.logprobs, use_lp), (got.entropy, use_h)) if use]
+        return torch.autograd.grad(outs, leaf, [g for g, use in ((g_lp, use_lp), (g_h, use_h)) if use])[0]
+
+    entropy = grad(inside, 0, 1)
+    assert torch.isfinite(entropy).all() and torch.equal(grad(tokens, 0, 1), entropy)
+    both = grad(tokens, 1, 1)
+    assert both[1:3].isnan().all() and torch.equal(both[3], entropy[3])  # -100 keeps the entropy's gradient
+    assert torch.equal(both[[0, 4]], grad(inside, 1, 1)[[0, 4]])
+    alone = grad(tokens, 1, 0)
+    assert alone[1:3].isnan().all() and (alone[3] == 0).all()
