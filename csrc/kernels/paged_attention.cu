@@ -33,10 +33,10 @@
 // Codes are exact in f16: e4m3 by one cvt, int8 as 1152 + c by one byte permute, less 1152. Queries are
 // scaled by a power of two to a row maximum in [1, 2) before they are rounded to f16: a bf16 value keeps all its bits
 // unless it is 2^-14 of the row's largest. P is rounded to f16 (11 bits, against 8 of bf16), sums
-// stay fp32. The key scale multiplies the fp32 score. O is held in multiples of a unit, the
-// largest value scale met: P is multiplied by (scale / unit) before it is rounded, and where that
-// leaves [2^-10, 1] the unit becomes this block's scale and O is rescaled, so that small values
-// keep their bits beside large ones.
+// stay fp32. The key scale multiplies the fp32 score. What is rounded is the product of P and the block's value scale, in
+// multiples of a unit of the row's own: a second running maximum, of score + log2(value scale), which moves like
+// the first (of the scores, for the sum of P). So each product keeps its 11 bits whatever ranges the row's blocks have, and
+// one that is lost is below 2^-24 of the row's largest.
 //
 // Measured (one B200, copy rate 6.54 TB/s): 16 requests of 4000 to 40000 tokens, 8 kv heads, 4 query
 // heads each, int8: 100 us for 632 MB (97 % of the copy rate); 100 requests of 1 to 4096 tokens, 12 heads,
@@ -69,7 +69,8 @@ constexpr int kStage = 2 * kHalf;
 constexpr int kStages = 2;      // one is read while the other is filled
 constexpr int kPart = D + 4;    // floats of a row's part, in whole 16 bytes
 constexpr float kLazy = 8.f;    // a running maximum may lag by 2^8: P stays below 256 in f16
-constexpr float kLeast = 0x1p-10f, kFar = 0x1p-60f;  // P times something between these changes the unit
+constexpr float kNoUnit = 1e30f;  // in place of log2(2^m / O's unit) before a value was met: O is 0
+constexpr float kMostRatio = 126.f;  // where 2^m / unit * scale is larger, P is 0
 
 struct AttnArgs {
   const __nv_bfloat16* q;
@@ -189,6 +190,16 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
 __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
   const __half2 v = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ float log2_of(float x) {
+  float y;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float min_nan(float a, float b) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
 }
 __device__ __forceinline__ uint32_t word(const uint4& v, int j) {
   return j == 0 ? v.x : j == 1 ? v.y : j == 2 ? v.z : v.w;
@@ -365,9 +376,11 @@ __global__ void __launch_bounds__(kThreads, 3) paged_attention_kernel(const Attn
     const int least = a.causal ? len - n + r0 / a.G + 1 : len;
 
     float o[NT][8][4] = {}, m[NT][2] = {}, l[NT][2] = {};
-    int none = (1 << 2 * NT) - 1;            // columns that have no maximum yet
-    float unit = 0.f, inv_unit = INFINITY;  // O is held in multiples of this
-    int last = -1;                          // the stage read last
+    float to_unit[NT][2];          // log2(2^m / unit), O of a column held in multiples of its unit
+    int none = (1 << 2 * NT) - 1;  // columns that have no maximum yet
+    int last = -1;                 // the stage read last
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) to_unit[nt][0] = to_unit[nt][1] = kNoUnit;
 
     for (int u = u0; u < u1; ++u) {
       const int kb = u * kUnitKeys + warp * kKeys;
@@ -433,36 +446,47 @@ __global__ void __launch_bounds__(kThreads, 3) paged_attention_kernel(const Attn
             for (int c = 0; c < 4; ++c)
               if (kb + half * 16 + g + (c >> 1) * 8 >= limit[nt][c & 1]) s[half][nt][c] = -INFINITY;
       }
-      float up[NT][2];
+      const float vlog[2] = {log2_of(scale.y), log2_of(scale.w)};
+      float up[2][NT][2];
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
+      for (int half = 0; half < 2; ++half)
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          up[nt][c] = fmaxf(fmaxf(s[0][nt][c], s[0][nt][c + 2]), fmaxf(s[1][nt][c], s[1][nt][c + 2]));
-          raise |= up[nt][c] > kLazy;
-        }
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            up[half][nt][c] = fmaxf(s[half][nt][c], s[half][nt][c + 2]);
+            raise |= fmaxf(up[half][nt][c], up[half][nt][c] + (vlog[half] + to_unit[nt][c])) > kLazy;
+          }
       if (__any_sync(~0u, raise)) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
           float alpha[2];
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
-            float by = up[nt][c];
-            by = fmaxf(by, __shfl_xor_sync(~0u, by, 4));
-            by = fmaxf(by, __shfl_xor_sync(~0u, by, 8));
-            by = fmaxf(by, __shfl_xor_sync(~0u, by, 16));
+            float by = fmaxf(up[0][nt][c], up[1][nt][c]);
+            float most_v = fmaxf(up[0][nt][c] + vlog[0], up[1][nt][c] + vlog[1]);
+#pragma unroll
+            for (int off = 4; off < 32; off *= 2) {
+              by = fmaxf(by, __shfl_xor_sync(~0u, by, off));
+              most_v = fmaxf(most_v, __shfl_xor_sync(~0u, most_v, off));
+            }
             const int bit = 1 << (nt * 2 + c);
-            alpha[c] = 1.f;
             if (none & bit ? by > -INFINITY : by > 0.f) {
-              if (!(none & bit)) alpha[c] = fast_exp2(-by);
+              if (!(none & bit)) l[nt][c] *= fast_exp2(-by);
               none &= ~bit;
               m[nt][c] += by;
-              l[nt][c] *= alpha[c];
+              to_unit[nt][c] += by;
+              most_v -= by;
 #pragma unroll
               for (int half = 0; half < 2; ++half) {
                 s[half][nt][c] -= by;
                 s[half][nt][c + 2] -= by;
               }
+            }
+            alpha[c] = 1.f;
+            if (most_v > -INFINITY && most_v + to_unit[nt][c] > 0.f) {  // the unit becomes the largest product
+              alpha[c] = fast_exp2(-most_v - to_unit[nt][c]);
+              to_unit[nt][c] = -most_v;
             }
           }
 #pragma unroll
@@ -477,31 +501,18 @@ __global__ void __launch_bounds__(kThreads, 3) paged_attention_kernel(const Attn
 
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
-        const float vs = half ? scale.w : scale.y;
-        const bool any = vs != 0.f && kb + half * 16 < most;  // else P or V is zero
-        float ratio = any ? vs * inv_unit : 0.f;
-        if (any && (!(ratio <= 1.f) || (ratio < kLeast && ratio > kFar))) {
-          const float to = unit / vs;
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int mt = 0; mt < 8; ++mt)
-#pragma unroll
-              for (int c = 0; c < 4; ++c) o[nt][mt][c] *= to;
-          unit = vs;
-          inv_unit = 1.f / vs;
-          ratio = 1.f;
-        }
         uint32_t pb[NT][2];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          float p[4];
+          float p[4], ratio[2];
+#pragma unroll
+          for (int c = 0; c < 2; ++c) ratio[c] = fast_exp2(min_nan(vlog[half] + to_unit[nt][c], kMostRatio));
 #pragma unroll
           for (int c = 0; c < 4; ++c) p[c] = fast_exp2(s[half][nt][c]);
           l[nt][0] += p[0] + p[2];
           l[nt][1] += p[1] + p[3];
-          pb[nt][0] = transpose8x8(pack_f16x2(p[0] * ratio, p[1] * ratio));
-          pb[nt][1] = transpose8x8(pack_f16x2(p[2] * ratio, p[3] * ratio));
+          pb[nt][0] = transpose8x8(pack_f16x2(p[0] * ratio[0], p[1] * ratio[1]));
+          pb[nt][1] = transpose8x8(pack_f16x2(p[2] * ratio[0], p[3] * ratio[1]));
         }
         const uint4 v0 = codes(vp + half * kHalf), v1 = codes(vp + half * kHalf + D), v2 = codes(vp + half * kHalf + 8 * D),
                     v3 = codes(vp + half * kHalf + 9 * D);
@@ -539,6 +550,7 @@ __global__ void __launch_bounds__(kThreads, 3) paged_attention_kernel(const Attn
             s_m[warp][r] = none >> (nt * 2 + c) & 1 ? -INFINITY : m[nt][c];
             s_l[warp][r] = sum;
           }
+          const float unit = fast_exp2(-to_unit[nt][c]);
           float4* to = reinterpret_cast<float4*>(mine + r * D + g * 16);
 #pragma unroll
           for (int k = 0; k < 4; ++k)

@@ -1,0 +1,114 @@
+"""Paged attention where the value ranges of a request's blocks, or of its rows' futures, differ widely.
+
+The kernel multiplies a softmax weight by its block's value scale, relative to the largest such product of the
+row so far, before it rounds it to f16: each product that counts is good to 2^-11 of itself, and what is lost altogether is
+below 2^-24 of the largest. exp2 is good to 2^-21, and scores of magnitude 100 carry 2^-14 of rounding into it. With the
+output's own rounding to bf16 that makes 2^-8 |o| + 2^-10 sum p |v|.
+"""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+TYPES = [torch.int8, torch.float8_e4m3fn]
+
+
+def _i32(values, device):
+    return torch.tensor(values, dtype=torch.int32, device=device)
+
+
+def _request(device, dtype, heads, size, lengths):
+    """A cache of ones, scales 1, and the plan of the last token of each request."""
+    from hrm_text_b200.ops.paged import BlockTables, PagedKV8
+    most = max(lengths)
+    bt = BlockTables(sum(-(-n // size) for n in lengths), size, len(lengths), -(-most // size), device)
+    cache = PagedKV8.create(bt.free.numel(), size, heads, dtype, device)
+    bt.step(_i32([n - 1 for n in lengths], device), sum(lengths) - len(lengths))
+    plan = bt.step(_i32([1] * len(lengths), device), len(lengths), max_new=1)
+    bt.check()
+    for scales in (cache.key_scales, cache.value_scales):
+        scales.fill_(1.0)
+    return bt, cache, plan
+
+
+def _bound(out, q, cache, plan, causal=True):
+    from hrm_text_b200.models.paged import paged_attention_reference
+    want = paged_attention_reference(q.double(), cache, plan, causal, dtype=torch.float64)
+    mass = paged_attention_reference(q.double(), cache._replace(values=cache.values.float().abs()), plan, causal, dtype=torch.float64)
+    excess = (out.double() - want).abs() - (2.0 ** -8 * want.abs() + 2.0 ** -10 * mass)
+    assert torch.isfinite(out.float()).all() and excess.max() <= 0, float((excess / mass).max())
+
+
+# a query of sqrt(128) in dim 0 makes the first code of a key its score (natural logarithm)
+def _query(rows, heads, device):
+    q = torch.zeros(rows, heads, 128, device=device)
+    q[:, :, 0] = math.sqrt(128)
+    return q.bfloat16()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("seed", range(4))
+def test_weights_and_ranges_against_each_other(cuda_device, dtype, seed):
+    """Blocks whose scores differ by 70 and whose value scales by 2^120: any of them may decide a row."""
+    from hrm_text_b200.ops.paged import paged_attention
+    g = torch.Generator(device=cuda_device).manual_seed(seed)
+    lengths = [700, 33, 4000, 1]
+    bt, cache, plan = _request(cuda_device, dtype, 3, 16, lengths)
+    blocks = cache.keys.shape[0]
+    score = torch.randint(-33, 34, (blocks, 3, 1), generator=g, device=cuda_device)
+    codes = torch.randint(-100, 101, cache.values.shape, generator=g, device=cuda_device)
+    cache.values.copy_(codes.to(dtype))
+    cache.keys[..., 0] = (score + torch.randint(-2, 3, (blocks, 3, 16), generator=g, device=cuda_device)).to(dtype)
+    cache.value_scales.copy_(torch.exp2(torch.randint(-60, 61, (blocks, 3), generator=g, device=cuda_device).float()))
+    q = _query(4, 3, cuda_device)
+    _bound(paged_attention(q, cache, plan), q, cache, plan)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_all_the_weight_on_small_values(cuda_device, dtype):
+    """Blocks of values around 2^-80 with all the weight, among blocks of ordinary values with none."""
+    from hrm_text_b200.ops.paged import paged_attention
+    bt, cache, plan = _request(cuda_device, dtype, 2, 16, [640, 640])
+    cache.values.copy_(torch.full_like(cache.values, 64.0, dtype=torch.float32).to(dtype))
+    for i in range(2):
+        chosen = bt.tables[i, 5 + 13 * i].long()
+        cache.value_scales[chosen] = 2.0 ** -80
+        cache.keys[chosen, :, :, 0] = torch.tensor(96.0).to(dtype).to(cuda_device)
+    q = _query(2, 2, cuda_device)
+    out = paged_attention(q, cache, plan)
+    assert ((out.double() / (64 * 2.0 ** -80) - 1).abs() <= 2.0 ** -7).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_ranges_that_fall_again_and_again(cuda_device, dtype):
+    """Values of 2^100, 2^50, 1 and 2^-50 in a request's order: the first decide, and nothing overflows on the way."""
+    from hrm_text_b200.ops.paged import paged_attention
+    bt, cache, plan = _request(cuda_device, dtype, 10, 16, [512] * 60)
+    cache.values.copy_(torch.full_like(cache.values, 96.0, dtype=torch.float32).to(dtype))
+    for i in range(60):
+        for unit, e in enumerate((100, 50, 0, -50)):
+            cache.value_scales[bt.tables[i, 8 * unit:8 * unit + 8].long()] = 2.0 ** e
+    q = _query(60, 10, cuda_device)
+    _bound(paged_attention(q, cache, plan), q, cache, plan)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_many_small_weights_of_small_values(cuda_device, dtype):
+    """Equal products of a small weight and a small scale round alike, so their error does not average out: the
+    result is of values around 2^-3 with weights of e^-7 each, after a block of large values with no weight."""
+    from hrm_text_b200.ops.paged import paged_attention
+    lengths = [1024] * 50
+    bt, cache, plan = _request(cuda_device, dtype, 10, 16, lengths)
+    cache.values.copy_(torch.full_like(cache.values, 96.0, dtype=torch.float32).to(dtype))
+    cache.keys[..., 0] = torch.tensor(-7.0).to(dtype).to(cuda_device)
+    cache.value_scales.fill_(16.45 * 2.0 ** -24 * math.exp(7.0))
+    first = bt.tables[:, :8].long().flatten()
+    cache.value_scales[first] = 1.0
+    cache.keys[first, :, :, 0] = torch.tensor(-60.0).to(dtype).to(cuda_device)
+    second = bt.tables[:, 8:16].long().flatten()   # each sixteen keys' first has the largest score and no value
+    cache.keys[second, :, 0, 0] = torch.tensor(0.0).to(dtype).to(cuda_device)
+    cache.values[second, :, 0] = torch.tensor(0.0).to(dtype).to(cuda_device)
+    q = _query(50, 10, cuda_device)
+    _bound(paged_attention(q, cache, plan), q, cache, plan)
