@@ -502,6 +502,7 @@ __global__ void __launch_bounds__(kThreads, 3) paged_attention_kernel(const Attn
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
         uint32_t pb[NT][2];
+        const bool poisoned = vlog[half] != vlog[half];  // a block whose value scale is NaN
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
           float p[4], ratio[2];
@@ -511,8 +512,14 @@ __global__ void __launch_bounds__(kThreads, 3) paged_attention_kernel(const Attn
           for (int c = 0; c < 4; ++c) p[c] = fast_exp2(s[half][nt][c]);
           l[nt][0] += p[0] + p[2];
           l[nt][1] += p[1] + p[3];
-          pb[nt][0] = transpose8x8(pack_f16x2(p[0] * ratio[0], p[1] * ratio[1]));
-          pb[nt][1] = transpose8x8(pack_f16x2(p[2] * ratio[0], p[3] * ratio[1]));
+#pragma unroll
+          for (int c = 0; c < 4; ++c) p[c] *= ratio[c & 1];
+          if (poisoned) {  // not for the rows that do not see it
+#pragma unroll
+            for (int c = 0; c < 4; ++c) p[c] = s[half][nt][c] == -INFINITY ? 0.f : NAN;
+          }
+          pb[nt][0] = transpose8x8(pack_f16x2(p[0], p[1]));
+          pb[nt][1] = transpose8x8(pack_f16x2(p[2], p[3]));
         }
         const uint4 v0 = codes(vp + half * kHalf), v1 = codes(vp + half * kHalf + D), v2 = codes(vp + half * kHalf + 8 * D),
                     v3 = codes(vp + half * kHalf + 9 * D);

@@ -130,10 +130,13 @@ def paged_attention_reference(query: Tensor, cache: PagedKV8, plan: StepPlan, ca
                 for c, s in ((cache.keys, cache.key_scales), (cache.values, cache.value_scales)))
         q = query[cu[i]:cu[i + 1]].to(dtype).view(n, heads, group, 128)
         a = torch.einsum("nhgd,hkd->hngk", q, k) / math.sqrt(128)
-        if causal:
-            last = torch.arange(length - n, length, device=a.device)
-            a = a.masked_fill((torch.arange(length, device=a.device)[None] > last[:, None])[None, :, None], -math.inf)
-        out[cu[i]:cu[i + 1]] = torch.einsum("hngk,hkd->nhgd", a.softmax(-1), v).reshape(n, heads * group, 128)
+        last = torch.arange(length - n, length, device=a.device) if causal else torch.full((n,), length - 1, device=a.device)
+        unseen = torch.arange(length, device=a.device)[None] > last[:, None]
+        a = a.masked_fill(unseen[None, :, None], -math.inf)
+        # a NaN value is one for the rows that see it: a weight of zero times NaN would be for all
+        poison = v.isnan().any(-1).to(dtype) @ (~unseen).t().to(dtype) > 0  # [heads, n]
+        o = torch.einsum("hngk,hkd->nhgd", a.softmax(-1), v.nan_to_num(0.0, math.inf, -math.inf))
+        out[cu[i]:cu[i + 1]] = o.masked_fill(poison.t()[:, :, None, None], math.nan).reshape(n, heads * group, 128)
     if gate is not None:
         out = out * torch.sigmoid(gate.to(dtype))
     return out.to(query.dtype)

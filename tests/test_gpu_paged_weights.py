@@ -112,3 +112,35 @@ def test_many_small_weights_of_small_values(cuda_device, dtype):
     cache.values[second, :, 0] = torch.tensor(0.0).to(dtype).to(cuda_device)
     q = _query(50, 10, cuda_device)
     _bound(paged_attention(q, cache, plan), q, cache, plan)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("where", ["key", "value"])
+def test_nan_does_not_reach_earlier_tokens(cuda_device, dtype, where):
+    """A NaN token poisons its own block; a token before that block does not see it, with any neighbours in its tile."""
+    from hrm_text_b200.models.paged import paged_append_reference, paged_attention_reference
+    from hrm_text_b200.ops.paged import BlockTables, PagedKV8, paged_append, paged_attention
+    torch.manual_seed(7)
+    for old, new in ((14, 3), (127, 2), (30, 7), (300, 6)):
+        sides = []
+        kv = torch.randn(old + new, 2, 2, 128).bfloat16()
+        at = -(-(old + 1) // 16) * 16              # the first token of the block after the first new one's
+        kv[at, 0 if where == "key" else 1, 0, 3] = math.nan
+        for dev in (cuda_device, torch.device("cpu")):
+            bt = BlockTables(64, 16, 1, 40, dev)
+            cache = PagedKV8.create(64, 16, 2, dtype, dev)
+            append = paged_append if dev == cuda_device else paged_append_reference
+            for a, b in ((0, old), (old, old + new)):
+                plan = bt.step(_i32([b - a], dev), b - a)
+                append(kv[a:b, 0].to(dev), kv[a:b, 1].to(dev), cache, plan)
+            sides.append((cache, plan))
+        q = torch.randn(new, 2, 128).bfloat16()
+        out = paged_attention(q.to(cuda_device), *sides[0]).cpu()
+        want = paged_attention_reference(q.double(), *sides[1], dtype=torch.float64)
+        before = at - old
+        assert 0 < before < new and torch.isfinite(want[:before]).all() and torch.isfinite(want[:, 1]).all()
+        assert torch.isfinite(out[:before]).all() and torch.isfinite(out[:, 1]).all()
+        assert out[before:, 0].isnan().all() and want[before:, 0].isnan().all()
+        ok = torch.isfinite(want)
+        top = float(kv[:, 1].float().abs().nan_to_num(0.0).max()) * 1.07  # no read-back value is larger
+        assert ((out.double() - want)[ok].abs() <= (2.0 ** -8 * want.abs() + 2.0 ** -10 * top)[ok]).all()

@@ -3,7 +3,8 @@ import math
 
 import torch
 
-from hrm_text_b200.models.paged import token_logprobs_reference
+from hrm_text_b200.models.paged import paged_append_reference, paged_attention_reference, token_logprobs_reference
+from hrm_text_b200.ops.paged import BlockTables, PagedKV8
 
 
 def test_likeliest_order_is_nan_then_infinity_then_the_lowest_id():
@@ -12,3 +13,18 @@ def test_likeliest_order_is_nan_then_infinity_then_the_lowest_id():
     for dtype in (torch.float32, torch.float64):
         ids = token_logprobs_reference(rows.to(dtype), torch.zeros(3, dtype=torch.long), 5)[2]
         assert ids.tolist() == [[2, 4, 0, 3, 1], [0, 1, 4, 2, 3], [0, 1, 3, 4, 2]]
+
+
+def test_attention_oracle_keeps_nan_from_earlier_tokens():
+    torch.manual_seed(0)
+    bt, cache = BlockTables(4, 16, 1, 4), PagedKV8.create(4, 16, 2)
+    x = torch.randn(17, 2, 128)
+    value = x.clone()
+    value[16, 0, 5] = math.nan
+    paged_append_reference(x[:14], value[:14], cache, bt.step(torch.tensor([14], dtype=torch.int32), 14))
+    plan = bt.step(torch.tensor([3], dtype=torch.int32), 3)
+    paged_append_reference(x[14:], value[14:], cache, plan)
+    q = torch.randn(3, 4, 128)
+    out = paged_attention_reference(q, cache, plan)
+    assert torch.isfinite(out[:2]).all() and torch.isfinite(out[:, 2:]).all() and out[2, :2].isnan().all()
+    assert paged_attention_reference(q, cache, plan, causal=False)[:, :2].isnan().all()
