@@ -90,7 +90,8 @@ struct AttnArgs {
   long g_st, g_sh;
   __nv_bfloat16* out;  // [T, Hq, 128]
   long o_st;
-  float* part;  // [2 * workers][tiles][8 * NT][kPart]: output, maximum, sum
+  float* part;     // [2 * workers][tiles][8 * NT][kPart]: output, maximum, sum
+  int first_tile;  // of this launch
 };
 
 struct Found {
@@ -282,7 +283,7 @@ __global__ void __launch_bounds__(kThreads, 3) paged_attention_kernel(const Attn
   __shared__ __align__(16) uint32_t s_q[NT == 1 ? 1 : 8][32][NT * 2];  // queries, where registers are short
   __shared__ int s_part[kWarps];  // where in s_ring a warp's part of the merge is, -1: it has none
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, tg = lane & 3;
-  const int worker = blockIdx.x, tile = blockIdx.y, r0 = tile * ROWS, Hq = a.Hkv * a.G;
+  const int worker = blockIdx.x, tile = a.first_tile + blockIdx.y, r0 = tile * ROWS, Hq = a.Hkv * a.G;
   asm volatile("griddepcontrol.wait;" ::: "memory");               // this grid starts while the kernel before it ends
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the join may take its places; it waits for the end
 
@@ -294,6 +295,11 @@ __global__ void __launch_bounds__(kThreads, 3) paged_attention_kernel(const Attn
         *reinterpret_cast<uint4*>(a.out + t * a.o_st + c * 8) = make_uint4(0, 0, 0, 0);
   const long total = (long)units * a.Hkv, per = (total + gridDim.x - 1) / gridDim.x;
   if (per * worker >= total) return;
+  if (tile > 0) {  // the step's bound of new tokens may be far above what any request has
+    bool some = mine.n * a.G > r0;
+    for (int j = threadIdx.x + kThreads; j < a.R && !some; j += kThreads) some = (a.cu_new[j + 1] - a.cu_new[j]) * a.G > r0;
+    if (!__syncthreads_or(some)) return;
+  }
   Walk walk;
   walk.x = per * worker;
   walk.x_end = min(total, walk.x + per);
@@ -569,7 +575,7 @@ __global__ void __launch_bounds__(kThreads, 3) paged_attention_kernel(const Attn
     __syncthreads();
     const bool whole = u0 == 0 && u1 == walk.nu;
     // the part of a pair that starts here but ends elsewhere has the worker's second place
-    float* part = a.part + ((long)(2 * worker + (u0 == 0 ? 1 : 0)) * gridDim.y + tile) * ROWS * kPart;
+    float* part = whole ? nullptr : a.part + ((long)(2 * worker + (u0 == 0 ? 1 : 0)) * gridDim.y + tile) * ROWS * kPart;
     int from[kWarps];
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) from[w] = s_part[w];
@@ -741,11 +747,16 @@ template <bool FP8, int NT>
 void launch(AttnArgs a, int max_rows, const at::TensorOptions& opts) {
   constexpr int ROWS = 8 * NT, smem = kWarps * kStages * kStage;
   const int tiles = (max_rows + ROWS - 1) / ROWS;
-  TORCH_CHECK(tiles <= 65535, "paged_attention: too many new tokens for one request");
   C10_CUDA_CHECK(ensure_dynamic_smem((const void*)paged_attention_kernel<FP8, NT>, smem));
   // with many tiles (a request with many new tokens) fewer ranges a tile: the grid stays at about four waves,
   // the workspace under 32 MB
   const int resident = device_sm_count() * 3, workers = tiles <= 4 ? resident : std::max(1, 4 * resident / tiles);
+  if (workers == 1) {  // each tile in one CTA: no pair is cut, nothing is to be joined
+    constexpr int kMostTiles = 65535;  // of one launch
+    for (a.first_tile = 0; a.first_tile < tiles; a.first_tile += kMostTiles)
+      launch_early(paged_attention_kernel<FP8, NT>, dim3(1, std::min(tiles - a.first_tile, kMostTiles)), kThreads, smem, a);
+    return;
+  }
   const at::Tensor part = at::empty({2L * workers * tiles * ROWS * kPart}, opts.dtype(at::kFloat));
   a.part = part.data_ptr<float>();
   const dim3 grid(workers, tiles);
@@ -826,8 +837,9 @@ at::Tensor paged_attention(const at::Tensor& query, const at::Tensor& keys, cons
   }
   a.out = reinterpret_cast<__nv_bfloat16*>(out.data_ptr());
   a.o_st = out.stride(0);
-  const int64_t max_rows = std::min<int64_t>(max_new, T) * a.G;
-  TORCH_CHECK(max_rows < (1LL << 30), "paged_attention: too many rows");
+  // a request's new tokens fit its table
+  const int64_t max_rows = std::min<int64_t>({max_new, T, tables.size(1) * s}) * a.G;
+  TORCH_CHECK(max_rows < (1LL << 30), "paged_attention: too many query rows of a request for one call");
   TORCH_CHECK((tables.size(1) * s / kUnitKeys + kPairCost + 1) * H < (1LL << 31), "paged_attention: tables too wide");
   if (keys.scalar_type() == at::kFloat8_e4m3fn)
     launch_rows<true>(a, (int)std::max<int64_t>(max_rows, 1), query.options());

@@ -144,3 +144,59 @@ def test_nan_does_not_reach_earlier_tokens(cuda_device, dtype, where):
         ok = torch.isfinite(want)
         top = float(kv[:, 1].float().abs().nan_to_num(0.0).max()) * 1.07  # no read-back value is larger
         assert ((out.double() - want)[ok].abs() <= (2.0 ** -8 * want.abs() + 2.0 ** -10 * top)[ok]).all()
+
+
+def test_many_requests_in_one_step(cuda_device):
+    """A packed step of many requests whose plan does not know that each has few tokens: the grid and the workspace
+    stay bounded by what one request can have, and the result does not depend on it."""
+    from hrm_text_b200.ops.paged import BlockTables, PagedKV8, paged_append, paged_attention
+    torch.manual_seed(8)
+    requests, heads, group = 400, 2, 4
+    new = [(i * 7) % 48 + 12 for i in range(requests)]
+    rows = sum(new)
+    assert rows * group / 16 > 1776 * 1.5
+    bt = BlockTables(requests * 2, 64, requests, 300, cuda_device)
+    cache = PagedKV8.create(requests * 2, 64, heads, torch.int8, cuda_device)
+    plan = bt.step(_i32(new, cuda_device), rows)
+    x = torch.randn(rows, 2, heads, 128, device=cuda_device).bfloat16()
+    paged_append(x[:, 0], x[:, 1], cache, plan)
+    q = torch.randn(rows, heads * group, 128, device=cuda_device).bfloat16()
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    out = paged_attention(q, cache, plan)
+    torch.cuda.synchronize()
+    assert torch.cuda.max_memory_allocated() - before < (33 << 20) + out.numel() * 2
+    _bound(out, q, cache, plan)
+    tight = paged_attention(q, cache, plan._replace(max_new=max(new)))
+    _bound(tight, q, cache, plan)
+
+
+def test_half_a_million_rows_in_one_step(cuda_device):
+    """More nominal tiles than a launch's second grid dimension takes; no request has more than a thousand tokens."""
+    from hrm_text_b200.ops.paged import BlockTables, PagedKV8, paged_append, paged_attention
+    torch.manual_seed(9)
+    requests, group = 530, 2
+    new = [1000] * requests
+    rows = sum(new)
+    bt = BlockTables(requests * 8, 128, requests, -(-rows // 128), cuda_device)
+    cache = PagedKV8.create(requests * 8, 128, 1, torch.float8_e4m3fn, cuda_device)
+    plan = bt.step(_i32(new, cuda_device), rows)
+    bt.check()
+    assert rows * group / 16 > 65535
+    x = torch.randn(rows, 2, 1, 128, device=cuda_device).bfloat16()
+    paged_append(x[:, 0], x[:, 1], cache, plan)
+    q = torch.randn(rows, group, 128, device=cuda_device).bfloat16()
+    out = paged_attention(q, cache, plan)
+    tight = paged_attention(q, cache, plan._replace(max_new=1000))
+    assert torch.isfinite(out.float()).all()
+    for i in (0, 1, 263, 529):
+        part = slice(i * 1000, (i + 1) * 1000)
+        ids = bt.tables[i, :8].long()
+        k, v = ((c[ids].double() * s[ids].double()[..., None, None]).reshape(-1, 128)[:1000]
+                for c, s in ((cache.keys, cache.key_scales), (cache.values, cache.value_scales)))
+        a = torch.einsum("ngd,kd->gnk", q[part].double(), k) / math.sqrt(128)
+        a = a.masked_fill(torch.ones(1000, 1000, dtype=torch.bool, device=cuda_device).triu(1), -math.inf).softmax(-1)
+        o, mass = (a @ v).transpose(0, 1), (a @ v.abs()).transpose(0, 1)
+        for got in (out, tight):
+            assert ((got[part].double() - o).abs() <= 2.0 ** -8 * o.abs() + 2.0 ** -10 * mass).all()
