@@ -90,8 +90,8 @@ struct AttnArgs {
   long g_st, g_sh;
   __nv_bfloat16* out;  // [T, Hq, 128]
   long o_st;
-  float* part;     // [2 * workers][tiles][8 * NT][kPart]: output, maximum, sum
-  int first_tile;  // of this launch
+  float* part;  // [tiles][workers][2][8 * NT][kPart]: output, maximum, sum
+  int split;    // 0: the grid is workers x tiles; else CTAs that the step's tiles are given
 };
 
 struct Found {
@@ -103,6 +103,31 @@ __device__ __forceinline__ Found request_of(const AttnArgs& a, int j) {
   if (j >= a.R) return Found{j, 0, 0, 0, 0, 0};
   const int row_t = a.cu_new[j];
   return Found{j, a.cu_units[j], a.cu_units[j + 1], row_t, a.cu_new[j + 1] - row_t, a.kv_len[j]};
+}
+// Which of a tile's workers a CTA is. Few tiles: the grid says so. Otherwise the host knows only a bound of the tiles,
+// which may be far above what the step's largest request has: that is read here, and the workers of a tile follow.
+struct Place {
+  int workers, worker, tile;
+  bool none;
+};
+template <int ROWS>
+__device__ __forceinline__ Place place_of(const AttnArgs& a, const Found& mine) {
+  Place p{(int)gridDim.x, (int)blockIdx.x, (int)blockIdx.y, false};
+  if (a.split > 0) {
+    __shared__ int s_most[32];
+    int n = mine.n;
+    for (int j = threadIdx.x + blockDim.x; j < a.R; j += blockDim.x) n = max(n, a.cu_new[j + 1] - a.cu_new[j]);
+    n = __reduce_max_sync(~0u, n);
+    if ((threadIdx.x & 31) == 0) s_most[threadIdx.x >> 5] = n;
+    __syncthreads();
+    for (int w = 0; w < (int)blockDim.x / 32; ++w) n = max(n, s_most[w]);
+    const int tiles = max(1, (int)(((long)n * a.G + ROWS - 1) / ROWS));
+    p.workers = max(1, a.split / tiles);
+    p.worker = blockIdx.x % p.workers;
+    p.tile = blockIdx.x / p.workers;
+    p.none = p.tile >= tiles;
+  }
+  return p;
 }
 // The request whose part of the costs laid end to end holds position `x`; every thread of the CTA
 // calls it. `mine` is request_of(threadIdx.x).
@@ -283,25 +308,24 @@ __global__ void __launch_bounds__(kThreads, 3) paged_attention_kernel(const Attn
   __shared__ __align__(16) uint32_t s_q[NT == 1 ? 1 : 8][32][NT * 2];  // queries, where registers are short
   __shared__ int s_part[kWarps];  // where in s_ring a warp's part of the merge is, -1: it has none
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, tg = lane & 3;
-  const int worker = blockIdx.x, tile = a.first_tile + blockIdx.y, r0 = tile * ROWS, Hq = a.Hkv * a.G;
+  const int Hq = a.Hkv * a.G;
   asm volatile("griddepcontrol.wait;" ::: "memory");               // this grid starts while the kernel before it ends
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the join may take its places; it waits for the end
 
   const Found mine = request_of(a, threadIdx.x);
   const int units = a.cu_units[a.R], real_rows = a.cu_new[a.R];
-  if (tile == 0)  // rows of no request
-    for (long t = real_rows + worker; t < a.T; t += gridDim.x)
+  const Place place = place_of<ROWS>(a, mine);
+  if (place.none) return;
+  const int r0 = place.tile * ROWS;
+  if (r0 == 0)  // rows of no request
+    for (long t = real_rows + place.worker; t < a.T; t += place.workers)
       for (int c = threadIdx.x; c < Hq * D / 8; c += kThreads)
         *reinterpret_cast<uint4*>(a.out + t * a.o_st + c * 8) = make_uint4(0, 0, 0, 0);
-  const long total = (long)units * a.Hkv, per = (total + gridDim.x - 1) / gridDim.x;
-  if (per * worker >= total) return;
-  if (tile > 0) {  // the step's bound of new tokens may be far above what any request has
-    bool some = mine.n * a.G > r0;
-    for (int j = threadIdx.x + kThreads; j < a.R && !some; j += kThreads) some = (a.cu_new[j + 1] - a.cu_new[j]) * a.G > r0;
-    if (!__syncthreads_or(some)) return;
-  }
+  const long total = (long)units * a.Hkv, per = (total + place.workers - 1) / place.workers;
+  if (per * place.worker >= total) return;
+  const int slot = (place.tile * place.workers + place.worker) * 2;  // this CTA's two places in the workspace
   Walk walk;
-  walk.x = per * worker;
+  walk.x = per * place.worker;
   walk.x_end = min(total, walk.x + per);
   walk.at = find_request(a, walk.x, mine);
   Ahead ahead;
@@ -575,7 +599,7 @@ __global__ void __launch_bounds__(kThreads, 3) paged_attention_kernel(const Attn
     __syncthreads();
     const bool whole = u0 == 0 && u1 == walk.nu;
     // the part of a pair that starts here but ends elsewhere has the worker's second place
-    float* part = whole ? nullptr : a.part + ((long)(2 * worker + (u0 == 0 ? 1 : 0)) * gridDim.y + tile) * ROWS * kPart;
+    float* part = a.part + (long)(slot + (u0 == 0 ? 1 : 0)) * ROWS * kPart;
     int from[kWarps];
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) from[w] = s_part[w];
@@ -622,10 +646,11 @@ struct Join {
   static constexpr int ROWS = 8 * NT, kFew = 8, JW = kJoin / 32;
   const AttnArgs& a;
   long per;
-  int h, first, parts, rows, row_t, r0, tile;
+  int base, r0;  // the tile's first place in the workspace, its first row
+  int h, first, parts, rows, row_t;
 
   __device__ __forceinline__ const float* part(int w, int r) const {  // the first worker may start with the pair or before
-    return a.part + (((long)(2 * (first + w) + (w == 0 ? 1 : 0)) * gridDim.y + tile) * ROWS + r) * kPart;
+    return a.part + ((long)(base + 2 * (first + w) + (w == 0 ? 1 : 0)) * ROWS + r) * kPart;
   }
   // parts w0, w0 + step, ... of row r, four dims from d on, added under a common maximum
   template <int N>
@@ -723,10 +748,11 @@ struct Join {
 template <int NT>
 __global__ void __launch_bounds__(kJoin) paged_attention_join_kernel(const AttnArgs a) {
   const Found mine = request_of(a, threadIdx.x);
-  const int worker = blockIdx.x;
-  const long total = (long)a.cu_units[a.R] * a.Hkv, per = (total + gridDim.x - 1) / gridDim.x;
+  const Place place = place_of<8 * NT>(a, mine);
+  const int worker = place.worker;
+  const long total = (long)a.cu_units[a.R] * a.Hkv, per = (total + place.workers - 1) / place.workers;
   const long x = per * worker, x_end = min(total, x + per);
-  const bool some = x < x_end;
+  const bool some = x < x_end && !place.none && place.workers > 1;  // one worker's pairs are whole
   Found at{}, end{};
   if (some) {  // the pairs at both ends of the range; those between are whole
     at = find_request(a, x, mine);
@@ -735,8 +761,8 @@ __global__ void __launch_bounds__(kJoin) paged_attention_join_kernel(const AttnA
   asm volatile("griddepcontrol.wait;" ::: "memory");  // the parts are written; in every CTA, so this grid ends last
   if (!some) return;
   Join<NT> join{a, per};
-  join.tile = blockIdx.y;
-  join.r0 = blockIdx.y * Join<NT>::ROWS;
+  join.base = place.tile * place.workers * 2;
+  join.r0 = place.tile * Join<NT>::ROWS;
   join.pair(at, x, worker);
   const int cost = at.c1 - at.c0;
   const long in = x - (long)at.c0 * a.Hkv;
@@ -748,18 +774,14 @@ void launch(AttnArgs a, int max_rows, const at::TensorOptions& opts) {
   constexpr int ROWS = 8 * NT, smem = kWarps * kStages * kStage;
   const int tiles = (max_rows + ROWS - 1) / ROWS;
   C10_CUDA_CHECK(ensure_dynamic_smem((const void*)paged_attention_kernel<FP8, NT>, smem));
-  // with many tiles (a request with many new tokens) fewer ranges a tile: the grid stays at about four waves,
-  // the workspace under 32 MB
-  const int resident = device_sm_count() * 3, workers = tiles <= 4 ? resident : std::max(1, 4 * resident / tiles);
-  if (workers == 1) {  // each tile in one CTA: no pair is cut, nothing is to be joined
-    constexpr int kMostTiles = 65535;  // of one launch
-    for (a.first_tile = 0; a.first_tile < tiles; a.first_tile += kMostTiles)
-      launch_early(paged_attention_kernel<FP8, NT>, dim3(1, std::min(tiles - a.first_tile, kMostTiles)), kThreads, smem, a);
-    return;
-  }
-  const at::Tensor part = at::empty({2L * workers * tiles * ROWS * kPart}, opts.dtype(at::kFloat));
+  // up to four tiles: each is cut among as many CTAs as fit the SMs. More (a request with many new tokens, or a step
+  // that does not say how many one may have): four waves of CTAs among the tiles that the step turns out to have, at
+  // least one a tile. The workspace is under 32 MB either way.
+  const int resident = device_sm_count() * 3;
+  a.split = tiles <= 4 ? 0 : 4 * resident;
+  const at::Tensor part = at::empty({2L * (a.split ? a.split : resident * tiles) * ROWS * kPart}, opts.dtype(at::kFloat));
   a.part = part.data_ptr<float>();
-  const dim3 grid(workers, tiles);
+  const dim3 grid = a.split ? dim3(std::max(a.split, tiles)) : dim3(resident, tiles);
   launch_early(paged_attention_kernel<FP8, NT>, grid, kThreads, smem, a);
   launch_early(paged_attention_join_kernel<NT>, grid, kJoin, 0, a);
 }

@@ -200,3 +200,24 @@ def test_half_a_million_rows_in_one_step(cuda_device):
         o, mass = (a @ v).transpose(0, 1), (a @ v.abs()).transpose(0, 1)
         for got in (out, tight):
             assert ((got[part].double() - o).abs() <= 2.0 ** -8 * o.abs() + 2.0 ** -10 * mass).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_grid_follows_the_step(cuda_device, dtype):
+    """What the plan says of one request's new tokens bounds the grid only: the work is cut by what the step has, so
+    the same step gives the same bits with a loose bound and with a tight one."""
+    from hrm_text_b200.ops.paged import BlockTables, PagedKV8, paged_append, paged_attention
+    torch.manual_seed(11)
+    for new, width in (([65, 3, 0, 700, 1], 12), ([90] * 300, 20), ([0, 0, 130], 40)):
+        rows = sum(new) + 2
+        bt = BlockTables(sum(-(-n // 64) for n in new) + 1, 64, len(new), width, cuda_device)
+        cache = PagedKV8.create(bt.free.numel(), 64, 2, dtype, cuda_device)
+        plan = bt.step(_i32(new, cuda_device), rows)
+        bt.check()
+        x = torch.randn(rows, 2, 2, 128, device=cuda_device).bfloat16()
+        paged_append(x[:, 0], x[:, 1], cache, plan)
+        q = torch.randn(rows, 4, 128, device=cuda_device).bfloat16()
+        out = paged_attention(q, cache, plan)
+        assert (out[sum(new):] == 0).all()
+        _bound(out[:sum(new)], q[:sum(new)], cache, plan)
+        assert torch.equal(out, paged_attention(q, cache, plan._replace(max_new=max(new))))
