@@ -12,6 +12,9 @@
 //   truncate(keep)  L_i = min(L_i, keep_i); surplus blocks go back in the reverse order of
 //                   ranks, so a truncate to the lengths before a step undoes that step exactly.
 //
+// The state may have been restored or changed from outside: lengths outside the table and counts outside the stack
+// are a failure of either call, which then changes nothing; block ids are checked where the cache is read.
+//
 // Both are one launch and read no host value, so a captured decode step crosses block
 // boundaries by itself. Every CTA computes the prefix sums over the requests for itself (a few
 // loads a thread, in L2) instead of waiting for another kernel or CTA; the rows are spread over
@@ -39,7 +42,7 @@ constexpr int kRows = 4;            // rows of a step that a thread takes togeth
 constexpr int kMaxRequests = 8192;  // three prefix arrays of this many int32 in shared memory
 
 // status codes; the Python side names them
-enum StepStatus : int { kStepOk = 0, kStepPool = 1, kStepRows = 2, kStepLong = 3, kStepNegative = 4, kStepMaxNew = 5 };
+enum StepStatus : int { kStepOk = 0, kStepPool = 1, kStepRows = 2, kStepLong = 3, kStepNegative = 4, kStepMaxNew = 5, kStepState = 6 };
 
 struct Sums {
   long long a, b, c, d;
@@ -105,7 +108,7 @@ struct StepArgs {
   int* num_free;
   int* status;  // [code, request]
   int* done;
-  int R, MB, size_log2, rows, max_new, max_runs;
+  int R, MB, F, size_log2, rows, max_new, max_runs;  // F: places of the stack
   int* slots;
   int* positions;
   int* cu_new;
@@ -130,7 +133,12 @@ __global__ void __launch_bounds__(kThreads) paged_step_kernel(const StepArgs a) 
   int bad = kStepOk, bad_at = 0;
   for (int i = i0; i < i1; ++i) {
     const long long len = a.lengths[i], n = a.fresh[i];
-    const int code = n < 0 ? kStepNegative : n > a.max_new ? kStepMaxNew : len + n > ((long long)a.MB << a.size_log2) ? kStepLong : kStepOk;
+    const long long most = (long long)a.MB << a.size_log2;
+    const int code = len < 0 || len > most ? kStepState
+                     : n < 0               ? kStepNegative
+                     : n > a.max_new       ? kStepMaxNew
+                     : len + n > most      ? kStepLong
+                                           : kStepOk;
     if (code != kStepOk && bad == kStepOk) {
       bad = code;
       bad_at = i;
@@ -146,7 +154,7 @@ __global__ void __launch_bounds__(kThreads) paged_step_kernel(const StepArgs a) 
   // the same verdict in every CTA: a request's own fault before the whole step's
   __shared__ int s_bad, s_bad_at;
   if (tid == 0) {
-    s_bad = total.a > a.rows ? kStepRows : total.b > free_top ? kStepPool : kStepOk;
+    s_bad = free_top < 0 || free_top > a.F ? kStepState : total.a > a.rows ? kStepRows : total.b > free_top ? kStepPool : kStepOk;
     s_bad_at = -1;
   }
   __syncthreads();
@@ -254,7 +262,7 @@ __global__ void __launch_bounds__(kThreads) paged_step_kernel(const StepArgs a) 
 
 __global__ void __launch_bounds__(kThreads)
     paged_truncate_kernel(int* tables, long table_ld, int* lengths, const int* __restrict__ keep, int* free_stack,
-                          int* num_free, int* done, int R, int size_log2) {
+                          int* num_free, int* status, int* done, int R, int MB, int F, int size_log2) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
   extern __shared__ int s_rank[];  // [R] freed blocks of the requests before
   const int size = 1 << size_log2, tid = threadIdx.x;
@@ -263,8 +271,26 @@ __global__ void __launch_bounds__(kThreads)
   const auto blocks = [&](int n) { return (int)(((long long)n + size - 1) >> size_log2); };
   const auto kept = [&](int i) { return min(lengths[i], max(keep[i], 0)); };
   Sums mine{0, 0, 0, 0}, total;
-  for (int i = i0; i < i1; ++i) mine.a += blocks(lengths[i]) - blocks(kept(i));
+  int bad_at = R;
+  for (int i = i0; i < i1; ++i) {
+    mine.a += blocks(lengths[i]) - blocks(kept(i));
+    if (lengths[i] < 0 || lengths[i] > ((long long)MB << size_log2)) bad_at = min(bad_at, i);
+  }
   Sums at = block_exclusive(mine, total);
+  __shared__ int s_bad_at;  // R: no request is at fault
+  if (tid == 0) s_bad_at = R;
+  __syncthreads();
+  if (bad_at < R) atomicMin(&s_bad_at, bad_at);
+  __syncthreads();
+  // the same verdict in every CTA
+  const bool failed = s_bad_at < R || top < 0 || top > F || total.a > F - top;
+  if (failed) {
+    if (last_cta(done) && tid == 0 && status[0] == kStepOk) {
+      status[0] = kStepState;
+      status[1] = s_bad_at < R ? s_bad_at : -1;
+    }
+    return;
+  }
   for (int i = i0; i < i1; ++i) {
     s_rank[i] = (int)at.a;
     at.a += blocks(lengths[i]) - blocks(kept(i));
@@ -342,6 +368,7 @@ std::vector<at::Tensor> paged_step(const at::Tensor& tables, const at::Tensor& l
   a.done = done.data_ptr<int>();
   a.R = (int)R;
   a.MB = (int)tables.size(1);
+  a.F = (int)free_stack.numel();
   a.size_log2 = log2_of(block_size);
   a.rows = (int)rows;
   a.max_new = (int)std::min<int64_t>(max_new, INT32_MAX);
@@ -375,7 +402,8 @@ void paged_truncate(const at::Tensor& tables, const at::Tensor& lengths, const a
   const int grid = std::max(1, std::min((R + kWarps - 1) / kWarps, 2 * device_sm_count()));
   launch_early(paged_truncate_kernel, dim3(grid), kThreads, R * 4, tables.data_ptr<int>(), tables.stride(0),
                lengths.data_ptr<int>(), keep.data_ptr<int>(), free_stack.data_ptr<int>(), num_free.data_ptr<int>(),
-               done.data_ptr<int>(), R, log2_of(block_size));
+               status.data_ptr<int>(), done.data_ptr<int>(), R, (int)tables.size(1), (int)free_stack.numel(),
+               log2_of(block_size));
 }
 
 }  // namespace hrm

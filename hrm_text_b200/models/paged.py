@@ -28,13 +28,13 @@ def step_reference(tables: BlockTables, new_tokens: Tensor, rows: int, max_new: 
     blocks = lambda n: -(-n // size)  # noqa: E731
     code, at, most = 0, -1, tables.tables.shape[1] * size
     for i, (length, n) in enumerate(zip(lengths, new)):
-        fault = 4 if n < 0 else 5 if n > plan.max_new else 3 if length + n > most else 0
+        fault = 6 if not 0 <= length <= most else 4 if n < 0 else 5 if n > plan.max_new else 3 if length + n > most else 0
         if fault:
             code, at = fault, i
             break
     need = [max(0, blocks(length + n) - blocks(length)) for length, n in zip(lengths, new)]
     if not code:
-        code = 2 if sum(new) > rows else 1 if sum(need) > int(tables.num_free) else 0
+        code = 6 if not 0 <= int(tables.num_free) <= tables.free.numel() else 2 if sum(new) > rows else 1 if sum(need) > int(tables.num_free) else 0
     if code:
         new, need = [0] * len(new), [0] * len(new)
         if int(tables.status[0]) == 0:
@@ -71,6 +71,12 @@ def truncate_reference(tables: BlockTables, keep: Tensor) -> None:
     size = tables.block_size
     blocks = lambda n: -(-n // size)  # noqa: E731
     kept = torch.minimum(tables.lengths, keep.clamp_min(0))
+    wild = (tables.lengths < 0) | (tables.lengths > size * tables.tables.shape[1])
+    surplus = sum(blocks(n) - blocks(k) for k, n in zip(kept.tolist(), tables.lengths.tolist()))
+    if wild.any() or not 0 <= int(tables.num_free) <= tables.free.numel() - surplus:
+        if int(tables.status[0]) == 0:
+            tables.status.copy_(torch.tensor([6, int(wild.int().argmax()) if wild.any() else -1], dtype=torch.int32))
+        return
     gone = [(i, b) for i, (k, n) in enumerate(zip(kept.tolist(), tables.lengths.tolist())) for b in range(blocks(k), blocks(n))]
     top = int(tables.num_free)
     for rank, (i, b) in enumerate(gone):

@@ -33,11 +33,12 @@ UNIT_KEYS, PAIR_COST = 128, 3  # how attention work is counted (csrc/kernels/pag
 MAX_REQUESTS = 8192
 
 STATUS = {1: "the pool has too few free blocks", 2: "more new tokens than num_tokens", 3: "a request outgrows its table",
-          4: "a negative number of new tokens", 5: "a request has more new tokens than max_new"}
+          4: "a negative number of new tokens", 5: "a request has more new tokens than max_new",
+          6: "lengths outside the table or free blocks outside the stack (a state from outside)"}
 
 
 class OutOfBlocks(RuntimeError):
-    """A step could not be held; nothing of it was done."""
+    """A step could not be held, or a state could not be stepped or truncated; nothing of it was done."""
 
 
 class PagedKV8(NamedTuple):
@@ -166,7 +167,8 @@ class BlockTables:
             truncate_reference(self, keep)
 
     def check(self) -> None:
-        """Raise ``OutOfBlocks`` if a step since the last check did not fit (waits for the device)."""
+        """Raise ``OutOfBlocks`` if a step since the last check did not fit, or a call met a state that cannot be (waits for
+        the device)."""
         code, request = self.status.tolist()
         if code:
             self.status.zero_()

@@ -221,3 +221,49 @@ def test_grid_follows_the_step(cuda_device, dtype):
         assert (out[sum(new):] == 0).all()
         _bound(out[:sum(new)], q[:sum(new)], cache, plan)
         assert torch.equal(out, paged_attention(q, cache, plan._replace(max_new=max(new))))
+
+
+def _states():
+    """(lengths, free blocks, request at fault) that no steps lead to, for tables of 3 requests of 4 blocks and a pool of 8."""
+    return [([3, 65, 0], 6, 1), ([3, 0, -1], 6, 2), ([3, 2 ** 31 - 1, 0], 6, 1), ([-(2 ** 31), 70, 0], 6, 0), ([3, 0, 0], 9, -1),
+            ([3, 0, 0], -1, -1), ([3, 0, 0], 2 ** 31 - 1, -1)]
+
+
+@pytest.mark.parametrize("lengths,free,at", _states())
+def test_states_that_cannot_be_change_nothing(cuda_device, lengths, free, at):
+    from hrm_text_b200.ops.paged import BlockTables, OutOfBlocks
+    for dev in (cuda_device, torch.device("cpu")):
+        bt = BlockTables(8, 16, 3, 4, dev)
+        bt.step(_i32([3, 17, 0], dev), 20)
+        bt.lengths.copy_(_i32(lengths, dev))
+        bt.num_free.fill_(free)
+        before = [t.clone() for t in (bt.tables, bt.lengths, bt.free, bt.num_free)]
+        words = "outside" + (rf".*request {at}" if at >= 0 else "")
+        for call in (lambda: bt.step(_i32([1, 1, 1], dev), 3), lambda: bt.truncate(_i32([0, 0, 0], dev)),
+                     lambda: bt.truncate(_i32([1 << 30] * 3, dev))):
+            plan = call()
+            assert plan is None or (plan.slots == -1).all() and int(plan.num_runs) == 0
+            for t, was in zip((bt.tables, bt.lengths, bt.free, bt.num_free), before):
+                assert torch.equal(t, was)
+            with pytest.raises(OutOfBlocks, match=words):
+                bt.check()
+            bt.check()
+        bt.lengths.copy_(_i32([3, 17, 0], dev))
+        bt.num_free.fill_(5)
+        assert bt.step(_i32([1, 1, 1], dev), 3).slots.min() >= 0
+
+
+def test_a_full_stack_takes_no_more_blocks(cuda_device):
+    """A restored state in which blocks are both owned and free."""
+    from hrm_text_b200.ops.paged import BlockTables, OutOfBlocks
+    for dev in (cuda_device, torch.device("cpu")):
+        bt = BlockTables(8, 16, 3, 4, dev)
+        bt.step(_i32([3, 17, 0], dev), 20)
+        twin = BlockTables.restore(bt.tables, bt.lengths, bt.free, torch.full_like(bt.num_free, 6), 16)
+        twin.truncate(_i32([3, 0, 0], dev))          # two more fit exactly
+        twin.check()
+        assert int(twin.num_free) == 8 and twin.lengths.tolist() == [3, 0, 0]
+        twin.truncate(_i32([0, 0, 0], dev))
+        with pytest.raises(OutOfBlocks, match="outside"):
+            twin.check()
+        assert int(twin.num_free) == 8 and twin.lengths.tolist() == [3, 0, 0]

@@ -1,10 +1,11 @@
 """The paged cache's and the log probabilities' oracle and entry points at their limits, on the CPU."""
 import math
 
+import pytest
 import torch
 
 from hrm_text_b200.models.paged import paged_append_reference, paged_attention_reference, token_logprobs_reference
-from hrm_text_b200.ops.paged import BlockTables, PagedKV8
+from hrm_text_b200.ops.paged import BlockTables, OutOfBlocks, PagedKV8
 
 
 def test_likeliest_order_is_nan_then_infinity_then_the_lowest_id():
@@ -28,3 +29,17 @@ def test_attention_oracle_keeps_nan_from_earlier_tokens():
     out = paged_attention_reference(q, cache, plan)
     assert torch.isfinite(out[:2]).all() and torch.isfinite(out[:, 2:]).all() and out[2, :2].isnan().all()
     assert paged_attention_reference(q, cache, plan, causal=False)[:, :2].isnan().all()
+
+
+@pytest.mark.parametrize("lengths,free,at", [([3, 65, 0], 6, 1), ([3, 0, -1], 6, 2), ([3, 0, 0], 9, -1), ([3, 0, 0], -1, -1)])
+def test_states_that_cannot_be_change_nothing(lengths, free, at):
+    bt = BlockTables(8, 16, 3, 4)
+    bt.step(torch.tensor([3, 17, 0], dtype=torch.int32), 20)
+    bt.lengths.copy_(torch.tensor(lengths))
+    bt.num_free.fill_(free)
+    before = [t.clone() for t in (bt.tables, bt.lengths, bt.free, bt.num_free)]
+    for call in (lambda: bt.step(torch.ones(3, dtype=torch.int32), 3), lambda: bt.truncate(torch.zeros(3, dtype=torch.int32))):
+        call()
+        assert all(torch.equal(t, was) for t, was in zip((bt.tables, bt.lengths, bt.free, bt.num_free), before))
+        with pytest.raises(OutOfBlocks, match="outside" + (f".*request {at}" if at >= 0 else "")):
+            bt.check()
