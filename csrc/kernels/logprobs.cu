@@ -430,7 +430,7 @@ int row_threads(int64_t N, int64_t row_bytes) {
 }
 
 void check_logits(const at::Tensor& logits, const at::Tensor& tokens) {
-  TORCH_CHECK(logits.is_cuda() && logits.dim() == 2 && (logits.numel() == 0 || logits.stride(1) == 1) &&
+  TORCH_CHECK(logits.is_cuda() && logits.dim() == 2 && (logits.numel() == 0 || logits.size(1) == 1 || logits.stride(1) == 1) &&
                   (logits.scalar_type() == at::kFloat || logits.scalar_type() == at::kBFloat16),
               "token_logprobs: logits CUDA [rows, vocabulary], fp32 or bf16, rows contiguous");
   TORCH_CHECK(logits.size(1) >= 1 && logits.size(1) < (1LL << 31) - 16, "token_logprobs: vocabulary size");
@@ -497,7 +497,7 @@ void token_logprobs_bwd(const at::Tensor& logits, const at::Tensor& tokens, cons
                   stats.device() == logits.device(),
               "token_logprobs: statistics of the forward pass");
   TORCH_CHECK(grad.sizes() == logits.sizes() && grad.scalar_type() == logits.scalar_type() &&
-                  grad.device() == logits.device() && (grad.numel() == 0 || grad.stride(1) == 1),
+                  grad.device() == logits.device() && (grad.numel() == 0 || grad.size(1) == 1 || grad.stride(1) == 1),
               "token_logprobs: gradient like the logits");
   if (N == 0) return;
   c10::cuda::CUDAGuard guard(logits.device());

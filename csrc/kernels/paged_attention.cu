@@ -815,7 +815,8 @@ at::Tensor paged_attention(const at::Tensor& query, const at::Tensor& keys, cons
                 "paged_attention: fp32 scales [blocks, heads]");
   const auto rows_ok = [&](const at::Tensor& t) {
     return t.device() == keys.device() && t.scalar_type() == at::kBFloat16 && t.dim() == 3 && t.size(2) == D &&
-           (t.numel() == 0 || t.stride(2) == 1) && t.stride(0) % 8 == 0 && t.stride(1) % 8 == 0 &&
+           (t.numel() == 0 || t.stride(2) == 1) && (t.size(0) <= 1 || t.stride(0) % 8 == 0) &&
+           (t.size(1) <= 1 || t.stride(1) % 8 == 0) &&
            reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
   };
   TORCH_CHECK(rows_ok(query) && query.size(1) % H == 0 && query.size(1) > 0,

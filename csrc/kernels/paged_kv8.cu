@@ -259,7 +259,7 @@ void paged_append(const at::Tensor& key, const at::Tensor& value, const at::Tens
   for (const at::Tensor* t : {&key, &value})
     TORCH_CHECK(t->device() == keys.device() && t->scalar_type() == at::kBFloat16 && t->dim() == 3 && t->size(0) == T &&
                     t->size(1) == H && t->size(2) == D && (t->numel() == 0 || t->stride(2) == 1) &&
-                    t->stride(0) % 8 == 0 && t->stride(1) % 8 == 0 &&
+                    (T <= 1 || t->stride(0) % 8 == 0) && (H <= 1 || t->stride(1) % 8 == 0) &&
                     reinterpret_cast<uintptr_t>(t->data_ptr()) % 16 == 0,
                 "paged_append: key and value [T, heads, 128] bf16 on the cache's device, with 16-byte aligned rows");
   TORCH_CHECK(runs.device() == keys.device() && runs.scalar_type() == at::kInt && runs.dim() == 2 && runs.size(1) == 4 &&

@@ -93,3 +93,15 @@ def test_gradient_of_an_id_outside_the_vocabulary(cuda_device, dtype):
     assert torch.equal(both[[0, 4]], grad(inside, 1, 1)[[0, 4]])
     alone = grad(tokens, 1, 0)
     assert alone[1:3].isnan().all() and (alone[3] == 0).all()
+
+
+def test_strides_of_a_single_column(cuda_device):
+    from hrm_text_b200.ops.logprobs import token_logprobs
+    wide, _ = _rows(4, 10, torch.float32, cuda_device)
+    column = wide[:, ::3][:, :1]                 # [4, 1] with a column stride of 3, which nothing uses
+    assert column.stride(1) == 3
+    got = token_logprobs(column, torch.zeros(4, dtype=torch.long, device=cuda_device), 1)
+    assert (got.logprobs == 0).all() and (got.top_ids == 0).all()
+    leaf = column.detach().requires_grad_()
+    (grad,) = torch.autograd.grad(token_logprobs(leaf, torch.zeros(4, dtype=torch.long, device=cuda_device)).logprobs.sum(), leaf)
+    assert (grad == 0).all()

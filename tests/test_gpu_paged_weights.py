@@ -267,3 +267,17 @@ def test_a_full_stack_takes_no_more_blocks(cuda_device):
         with pytest.raises(OutOfBlocks, match="outside"):
             twin.check()
         assert int(twin.num_free) == 8 and twin.lengths.tolist() == [3, 0, 0]
+
+
+def test_strides_of_a_single_row(cuda_device):
+    from hrm_text_b200.ops.paged import BlockTables, PagedKV8, paged_append, paged_attention
+    torch.manual_seed(3)
+    bt = BlockTables(4, 16, 1, 4, cuda_device)
+    cache = PagedKV8.create(4, 16, 1, torch.int8, cuda_device)
+    plan = bt.step(_i32([1], cuda_device), 1)
+    wide = torch.randn(3, 259, device=cuda_device).bfloat16()
+    odd = torch.as_strided(wide, (1, 1, 128), (259, 131, 1))   # one row and one head: nothing steps by 259 or 131
+    paged_append(odd, odd, cache, plan)
+    out = paged_attention(odd, cache, plan, gate=odd)
+    want = odd.contiguous().float()
+    assert ((out.float() - want * torch.sigmoid(want)).abs() <= 0.02).all()
