@@ -105,3 +105,70 @@ def test_strides_of_a_single_column(cuda_device):
     leaf = column.detach().requires_grad_()
     (grad,) = torch.autograd.grad(token_logprobs(leaf, torch.zeros(4, dtype=torch.long, device=cuda_device)).logprobs.sum(), leaf)
     assert (grad == 0).all()
+
+
+def _threads(n, v, dtype, device):
+    sms = torch.cuda.get_device_properties(device).multi_processor_count
+    return 1024 if n <= 2 * sms else 64 if v * dtype.itemsize < 8192 else 128
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("v", [1, 5, 511, 1001, 2047, 4097, 32003, 32768, 151937])
+def test_many_rows_match_64_bits(cuda_device, dtype, v):
+    """More rows than are given 1024 threads each, at any start in memory, with masked, tied, NaN and ignored ones among them."""
+    from hrm_text_b200.models.paged import token_logprobs_reference
+    from hrm_text_b200.ops.logprobs import token_logprobs
+    n = 2 * torch.cuda.get_device_properties(cuda_device).multi_processor_count + 5
+    whole, tokens = _rows(n, v + 3, dtype, cuda_device, seed=v)
+    logits, tokens = whole[:, 1:v + 1], tokens % v
+    if v > 500:
+        logits[0, 5:] = -math.inf
+        logits[1] = -math.inf
+        logits[2] = torch.finfo(dtype).min
+        logits[3, ::7] = 12.0                    # more equal values than are ranked by counting
+        logits[4, v // 2] = math.nan
+        logits[5, 3] = math.inf
+        tokens[6], tokens[7] = -100, v
+    threads = _threads(n, v, dtype, cuda_device)
+    assert threads < 1024
+    r = (v / (2 * threads) + 40) * 2.0 ** -24 + 2.0 ** -18
+    for k in (0, min(5, v), min(64, v)):
+        got = token_logprobs(logits, tokens, k)
+        lp, h, ids, top = token_logprobs_reference(logits.double(), tokens, k)
+        log_s = torch.logsumexp(logits.double(), -1) - logits.double().amax(-1)
+        slack = (r * (1 + 2 * (log_s - h).abs()) + 2.0 ** -22 * h.abs()).nan_to_num(0.0, posinf=0.0)
+        torch.testing.assert_close(got.logprobs.double(), lp, rtol=2.0 ** -22, atol=r, equal_nan=True)
+        off = torch.where(h.isnan() & got.entropy.isnan(), 0.0, (got.entropy.double() - h).abs())
+        assert (off <= slack).all()
+        if k:
+            assert torch.equal(got.top_ids, ids)
+            torch.testing.assert_close(got.top_logprobs.double(), top, rtol=2.0 ** -22, atol=r, equal_nan=True)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("v", [5, 1001, 4097, 32768])
+def test_many_rows_gradient(cuda_device, dtype, v):
+    """From the statistics of the 64- and 128-thread forward kernels."""
+    from hrm_text_b200.ops.logprobs import token_logprobs
+    n = 2 * torch.cuda.get_device_properties(cuda_device).multi_processor_count + 5
+    logits, tokens = _rows(n, v, dtype, cuda_device, seed=v + 1)
+    logits[1, v // 2:] = -math.inf
+    logits[2] = -math.inf
+    tokens[0], tokens[1], tokens[3] = -100, 0, v - 1
+    g_lp, g_h = (torch.randn(n, device=cuda_device) for _ in range(2))
+    leaf = logits.clone().requires_grad_()
+    got = token_logprobs(leaf, tokens)
+    (grad,) = torch.autograd.grad((got.logprobs, got.entropy), leaf, (g_lp, g_h))
+    x = logits.double()
+    empty = (x == -math.inf).all(-1, keepdim=True)
+    logp = torch.log_softmax(torch.where(empty, torch.zeros_like(x), x), -1)
+    p = torch.where(empty, torch.zeros_like(x), logp.exp())
+    finite = torch.where(p > 0, logp, torch.zeros_like(logp))
+    h = -(p * finite).sum(-1, keepdim=True)
+    hot = torch.zeros_like(x).scatter_(1, tokens.clamp_min(0)[:, None], 1.0) * ((tokens >= 0)[:, None] & ~empty)
+    glp, gh = (g_lp.double() * (tokens >= 0))[:, None], g_h.double()[:, None]
+    want = glp * (hot - p) - gh * p * (finite + h)
+    r = (v / (2 * _threads(n, v, dtype, cuda_device)) + 40) * 2.0 ** -24 + 2.0 ** -17
+    half = 2.0 ** -8 if dtype == torch.bfloat16 else 0.0
+    bound = half * want.abs() + 4 * r * (glp.abs() + gh.abs()) * (p + hot) * (1 + h + finite.abs()) + 1e-12
+    assert grad.dtype == dtype and ((grad.double() - want).abs() <= bound).all()

@@ -281,3 +281,30 @@ def test_strides_of_a_single_row(cuda_device):
     out = paged_attention(odd, cache, plan, gate=odd)
     want = odd.contiguous().float()
     assert ((out.float() - want * torch.sigmoid(want)).abs() <= 0.02).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("chunk,group,size", [(700, 2, 64), (5000, 1, 16), (130, 7, 32)])
+def test_late_tiles_see_exactly_their_keys(cuda_device, dtype, chunk, group, size):
+    """Each new token's own key has nearly all its weight, and the next token's key would have as much if it were seen."""
+    from hrm_text_b200.ops.paged import BlockTables, PagedKV8, paged_append, paged_attention
+    torch.manual_seed(chunk)
+    heads, old = 2, [300, 1000]
+    bt = BlockTables(2 * (-(-(1000 + chunk) // size) + 1), size, 2, -(-(1000 + chunk) // size), cuda_device)
+    cache = PagedKV8.create(bt.free.numel(), size, heads, dtype, cuda_device)
+    k, v = (torch.randn(sum(old), heads, 128, device=cuda_device).bfloat16() for _ in range(2))
+    paged_append(k, v, cache, bt.step(_i32(old, cuda_device), sum(old)))
+    plan = bt.step(_i32([chunk, 1], cuda_device), chunk + 1)
+    bt.check()
+    k, v = (torch.randn(chunk + 1, heads, 128, device=cuda_device).bfloat16() for _ in range(2))
+    paged_append(k, v, cache, plan)
+    after = torch.cat([k[1:], k[:1]]).float()
+    q = (4 * (k.float() + after)).repeat_interleave(group, 1).bfloat16()
+    out = paged_attention(q, cache, plan)
+    own = v.float().repeat_interleave(group, 1)
+    assert ((out.float() - own).abs().mean((1, 2)) < 0.3).all()   # more than 0.5 where another token's value is mixed in
+    # with all the weight on one key the rest is lost below 2^-24 of it: 2^-8 |o| for bf16 and 2^-10 of the largest value
+    from hrm_text_b200.models.paged import paged_attention_reference
+    want = paged_attention_reference(q.double(), cache, plan, dtype=torch.float64)
+    top = float(cache.value_scales.max()) * (127 if dtype == torch.int8 else 448)
+    assert ((out.double() - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -10 * top).all()
