@@ -12,7 +12,8 @@
 On CUDA with labels, the head runs the fused kernel path
 (``hrm_text_b200.ops.loss.lm_head_cross_entropy``): the lm_head GEMM epilogue emits per-tile
 softmax statistics and argmax, so neither an fp32 copy of the logits nor a separate
-softmax pass exists.
+softmax pass exists. Without labels it returns bf16 logits, differentiable where gradients are
+enabled (``lm_head_logits``), for a loss of the caller's own.
 """
 from __future__ import annotations
 
@@ -85,9 +86,8 @@ class LMHead(nn.Module):
             w = self.lm_head.weight
             if fused_path(hidden) and hidden.dtype == torch.bfloat16 and w.dtype == torch.bfloat16 \
                     and w.shape[0] % 32 == 0:
-                from ..ops import gemm as G  # tcgen05 GEMM (inference logits)
-                flat = hidden.reshape(-1, hidden.shape[-1]).contiguous()
-                return new_carry, G.infer_linear(flat, w).view(*hidden.shape[:-1], w.shape[0])
+                from ..ops import loss as loss_ops  # tcgen05 GEMM
+                return new_carry, loss_ops.lm_head_logits(hidden, w)
             return new_carry, F.linear(hidden, w.to(hidden.dtype))
 
         labels = batch["labels"]

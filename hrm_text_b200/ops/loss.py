@@ -13,6 +13,9 @@ Backward, one vocabulary chunk of ``chunk`` rows of the head at a time (default 
 log-sum-exp; a dgrad GEMM adds ``dlogits_c @ W_c`` into an fp32 ``d hidden`` accumulator and
 an fp32 wgrad GEMM adds ``dlogits_c^T @ hidden`` into rows ``c`` of the head weight's
 ``main_grad``. Only one ``[T, chunk]`` bf16 buffer exists at a time.
+
+``lm_head_logits`` is the head without a loss, for losses of the caller's own (``ops.logprobs``): the bf16 logits,
+differentiable, with the same GEMMs.
 """
 from __future__ import annotations
 
@@ -75,3 +78,35 @@ def lm_head_cross_entropy(hidden: Tensor, weight: Tensor, labels: Tensor,
         raise ValueError("the vocabulary chunk must be a multiple of 256")
     loss_sum, correct = LMHeadCrossEntropy.apply(hidden, weight, labels, chunk)
     return loss_sum, correct.bool()
+
+
+class LMHeadLogits(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, hidden: Tensor, weight: Tensor):
+        ctx.save_for_backward(hidden, weight)
+        return G.infer_linear(hidden, weight)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        hidden, weight = ctx.saved_tensors
+        grad = grad.contiguous()
+        d_hidden = G.linear_dgrad(grad, weight) if ctx.needs_input_grad[0] else None
+        d_weight = None
+        if ctx.needs_input_grad[1]:
+            main = getattr(weight, "main_grad", None)
+            g_w = main if main is not None else torch.zeros(weight.shape, dtype=torch.float32, device=weight.device)
+            G.linear_wgrad_(grad, hidden, g_w)
+            d_weight = None if main is not None else g_w.to(weight.dtype)
+        return d_hidden, d_weight
+
+
+def lm_head_logits(hidden: Tensor, weight: Tensor) -> Tensor:
+    """bf16 ``hidden @ weight.T`` (``[..., H]`` and ``[V, H]``, ``V`` a multiple of 32), differentiable once where gradients are
+    enabled; the weight's gradient goes to its ``main_grad`` if it has one."""
+    flat = hidden.reshape(-1, hidden.shape[-1]).contiguous()
+    if torch.is_grad_enabled() and (flat.requires_grad or weight.requires_grad):
+        out = LMHeadLogits.apply(flat, weight)
+    else:
+        out = G.infer_linear(flat, weight)
+    return out.view(*hidden.shape[:-1], weight.shape[0])
