@@ -173,8 +173,8 @@ def paged_cached_attention(gate: Tensor, query: Tensor, key: Tensor, value: Tens
     """``sigmoid(gate) * attention`` of a step's packed rows (``[..., heads, 128]`` with as many rows as the plan).
 
     The step's keys and values go into the cache. A ``prompt`` (one request's tokens into an empty cache) attends to its own
-    keys and values as they are, bidirectionally unless the layer is causal; any other step's tokens attend to the
-    cache up to themselves.
+    keys and values as they are, bidirectionally unless the layer is causal, on CUDA by the PrefixLM kernel; any other
+    step's tokens attend to the cache up to themselves.
     """
     from .layers import prefixlm_attention_reference
     shape, dtype = query.shape, query.dtype
@@ -183,7 +183,14 @@ def paged_cached_attention(gate: Tensor, query: Tensor, key: Tensor, value: Tens
         gate, query, key, value = (t.to(torch.bfloat16) for t in (gate, query, key, value))
     append = paged_append if cache.keys.is_cuda else paged_append_reference
     append(key, value, cache, plan)
-    if prompt:
+    if prompt and cache.keys.is_cuda and query.shape == key.shape:  # the kernel reads the gate and applies it
+        from ..ops.attention import PackedSeq, attention_fwd
+        n, heads, _ = query.shape
+        i32 = dict(dtype=torch.int32, device=query.device)
+        packed = PackedSeq(plan.positions, torch.tensor([0, n], **i32), torch.tensor([0 if is_causal else n], **i32))
+        gqkv = torch.cat([gate, query, key, value], dim=1).view(n, -1)
+        out = attention_fwd(gqkv, heads, packed.schedule(is_causal))[1]
+    elif prompt:
         n = query.shape[0]
         cu, prefix = torch.tensor([0, n]), torch.tensor([n])
         out = torch.sigmoid(gate.float()).to(query.dtype) * prefixlm_attention_reference(query, key, value, is_causal, prefix, cu)
