@@ -27,6 +27,7 @@ from torch import Tensor, nn
 
 from ..config import PretrainConfig
 from ..data.dataset import V1DatasetMeta
+from ..ops.logprobs import MAX_TOP_K
 from ..ops.paged import MAX_REQUESTS, BlockTables
 from ..optim.adam_atan2 import AdamATan2
 from ..runtime.checkpoint import checkpoint_dir, latest_epoch
@@ -318,10 +319,14 @@ def generate_tokens(model: nn.Module, carry, prompts: Iterator[tuple[int, np.nda
     On a CUDA device with bf16 weights the decode step runs as one captured CUDA graph
     (``DecodeGraph``, ``PagedDecodeGraph``). ``kv_cache`` ``"int8"`` / ``"fp8"`` keeps the caches in 8 bits in
     blocks of ``block_size`` tokens from a pool of ``num_blocks`` (default: room for every slot at its longest;
-    with fewer, prompts wait until blocks are free). With ``logprobs=k`` yields ``(prompt_id, generated_ids,
+    with fewer, prompts wait until blocks are free). With ``logprobs=k`` (0 to 64) yields ``(prompt_id, generated_ids,
     GeneratedLogprobs)``, the ``k`` likeliest tokens among it."""
     device = device or next(model.parameters()).device
     dtype = next(model.parameters()).dtype
+    if logprobs is not None:
+        most = min(MAX_TOP_K, model.lm_head.weight.shape[0])
+        if not 0 <= logprobs <= most:
+            raise ValueError(f"logprobs must be 0 to {most} (or None), got {logprobs}")
     if kv_cache == "bf16":
         slots = _StaticSlots(model, carry, batch_size, max_tokens, dtype, device, use_cuda_graph)
     elif kv_cache in KV_CACHES:

@@ -1,11 +1,14 @@
 """The paged cache's and the log probabilities' oracle and entry points at their limits, on the CPU."""
 import math
 
+import numpy as np
 import pytest
 import torch
 
+from hrm_text_b200.inference.engine import generate_tokens
 from hrm_text_b200.models.paged import paged_append_reference, paged_attention_reference, token_logprobs_reference
 from hrm_text_b200.ops.paged import BlockTables, OutOfBlocks, PagedKV8
+from hrm_text_b200.runtime.factory import arch_preset, build_model
 
 
 def test_likeliest_order_is_nan_then_infinity_then_the_lowest_id():
@@ -43,3 +46,24 @@ def test_states_that_cannot_be_change_nothing(lengths, free, at):
         assert all(torch.equal(t, was) for t, was in zip((bt.tables, bt.lengths, bt.free, bt.num_free), before))
         with pytest.raises(OutOfBlocks, match="outside" + (f".*request {at}" if at >= 0 else "")):
             bt.check()
+
+
+def _model():
+    cfg = arch_preset("hrm", "L") | dict(vocab_size=48, max_seq_len=128, n_layers=2, hidden_size=128, num_heads=1)
+    torch.manual_seed(0)
+    return build_model(cfg).eval()
+
+
+@pytest.mark.parametrize("kv_cache", ["bf16", "int8"])
+@pytest.mark.parametrize("k", [-1, 49, 65])
+def test_alternatives_are_refused_before_a_prompt_is_taken(kv_cache, k):
+    taken = []
+
+    def prompts():
+        taken.append(0)
+        yield 0, np.arange(5)
+
+    with pytest.raises(ValueError, match="logprobs must be 0 to 48"):
+        next(generate_tokens(_model(), None, prompts(), max_tokens=32, max_generation=4, batch_size=1, stop_token=-1,
+                             kv_cache=kv_cache, logprobs=k))
+    assert not taken
