@@ -33,7 +33,7 @@ class SimpleEngine(BaseEngine):
 
     def generate(self, prompts: list[str], batch_size: int = 100, max_context: int = 1024,
                  max_tokens: Optional[int] = None, temperature: float = 0.0, condition: str = "direct",
-                 kv_cache: str = "bf16") -> list[str]:
+                 kv_cache: str = "bf16", block_size: int = 64, num_blocks: Optional[int] = None) -> list[str]:
         from hrm_text_b200.inference.engine import inference_generate
         max_tokens = max_context if max_tokens is None else max_tokens
         outputs = [""] * len(prompts)
@@ -44,7 +44,7 @@ class SimpleEngine(BaseEngine):
         except Exception:
             bar = None
         for pid, text in inference_generate(self.ckpt, work, max_context, max_tokens, batch_size, temperature,
-                                            kv_cache=kv_cache):
+                                            kv_cache=kv_cache, block_size=block_size, num_blocks=num_blocks):
             outputs[pid] = text
             if bar is not None:
                 bar.update()

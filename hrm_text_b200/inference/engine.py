@@ -11,9 +11,11 @@ Behaviour follows the reference's simple_inference_engine.py:
 * sampling is greedy for ``temp < 1e-5`` and Gumbel-max otherwise (:93-102).
 
 Every module call of the recurrent model has its own static cache (one per call and layer,
-``model.create_cache``). ``kv_cache="int8"`` or ``"fp8"`` holds keys and values in 8 bits in blocks that
-requests own only as far as they are filled (``ops.paged``); ``logprobs`` adds the log probability, entropy
-and likeliest alternatives of every generated token (``ops.logprobs``). Both are additions to the reference.
+``model.create_cache``). ``kv_cache="int8"`` or ``"fp8"`` holds keys and values in 8 bits in blocks of one
+pool (``ops.paged``). A prompt reserves the blocks of its own longest generation until it ends, so that a
+step never runs out; with ``num_blocks`` below every slot at its longest, as many prompts run together
+as fit. ``logprobs`` adds the log probability, entropy and likeliest alternatives of every generated token
+(``ops.logprobs``; of the bf16 logits that the token is drawn from). Both are additions to the reference.
 """
 from __future__ import annotations
 
@@ -404,10 +406,10 @@ def generate_tokens(model: nn.Module, carry, prompts: Iterator[tuple[int, np.nda
 
 def inference_generate(ckpt: InferenceCheckpoint, iterator: Iterator[tuple[int, tuple[str, str]]], max_tokens: int,
                        max_generation: int, batch_size: int, temp: float = 0.0, kv_cache: str = "bf16",
-                       block_size: int = 64) -> Generator[tuple[int, str], None, None]:
-    """Text in, text out: ``iterator`` yields ``(prompt_id, (condition, prompt))``."""
+                       block_size: int = 64, num_blocks: Optional[int] = None) -> Generator[tuple[int, str], None, None]:
+    """Text in, text out: ``iterator`` yields ``(prompt_id, (condition, prompt))``; the caches as in ``generate_tokens``."""
     stop = ckpt.tokenizer.convert_tokens_to_ids(ckpt.tokenizer_info["eoa"])
     tokenized = ((pid, ckpt.tokenize_prompt(*p)) for pid, p in iterator)
     for pid, toks in generate_tokens(ckpt.model, ckpt.carry, tokenized, max_tokens, max_generation, batch_size,
-                                     stop, temp, kv_cache=kv_cache, block_size=block_size):
+                                     stop, temp, kv_cache=kv_cache, block_size=block_size, num_blocks=num_blocks):
         yield pid, ckpt.decode_generation(toks, stop) if toks.size else ""

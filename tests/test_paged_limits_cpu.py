@@ -67,3 +67,40 @@ def test_alternatives_are_refused_before_a_prompt_is_taken(kv_cache, k):
         next(generate_tokens(_model(), None, prompts(), max_tokens=32, max_generation=4, batch_size=1, stop_token=-1,
                              kv_cache=kv_cache, logprobs=k))
     assert not taken
+
+
+class _Words:
+    """A tokenizer of numbers."""
+
+    def __call__(self, text, add_special_tokens):
+        return {"input_ids": [int(w) for w in text.split()]}
+
+    def decode(self, ids):
+        return " ".join(map(str, ids))
+
+    def convert_tokens_to_ids(self, token):
+        return -1
+
+
+def test_text_generation_shares_a_small_pool(monkeypatch):
+    """A pool of blocks for one request at its longest: the same texts as with room for all, from a smaller cache."""
+    import hrm_text_b200.inference.engine as engine
+    info = dict(boq="", eoq="", eoa="", condition_mapping={"direct": ""})
+    ckpt = engine.InferenceCheckpoint(_model(), None, _Words(), info)
+    prompts = ["3 1 4 1 5", "9 2 6", "5 3 5 8 9 7 9"]
+    pools = []
+    create = BlockTables.__init__
+    monkeypatch.setattr(BlockTables, "__init__", lambda self, num_blocks, *a: (pools.append(num_blocks), create(self, num_blocks, *a))[1])
+
+    def run(**kw):
+        return dict(engine.inference_generate(ckpt, ((i, ("direct", p)) for i, p in enumerate(prompts)), 32, 6, 3, kv_cache="int8",
+                                              block_size=16, **kw))
+
+    whole, small = run(), run(num_blocks=2)
+    assert whole == small and all(len(t.split()) == 6 for t in whole.values()) and pools == [6, 2]
+
+    from evaluation.engines import SimpleEngine
+    simple = SimpleEngine.__new__(SimpleEngine)
+    simple.ckpt = ckpt
+    assert simple.generate(prompts, 3, 32, 6, kv_cache="int8", block_size=16, num_blocks=2) == [whole[i] for i in range(3)]
+    assert pools == [6, 2, 2]
