@@ -14,17 +14,21 @@
 // groups, and k groups hold a value of at least the k-th largest of the groups' largest values, so
 // that value bounds the answer from below. The pass has noted the largest value of every 64 bytes:
 // those that reach the bound, few more than k, are read again, and their values at or above it
-// are ranked by counting. Rows with more such values than fit (long runs of equal ones) are
-// searched k times instead.
+// are ranked by counting. Rows with more such values than fit are searched k times instead: long runs of equal
+// values, and, because the bound is then minus infinity, rows above 12288 bf16 or 6144 fp32 logits in which a mask
+// leaves fewer than k of the groups a finite value (33 rows of 32768 bf16 with 30 tokens left, twenty
+// alternatives: 123 us, 6.6 unmasked).
 //
 // Gradient: dx_j = g_lp (1[j = t] - p_j) - g_H p_j (log p_j + H), one read and one write.
 //
-// Measured (one B200, copy rate 6.54 TB/s): 8192 rows of 32768 bf16 90 us forward (91 % of the copy
-// rate; 100 us with the likeliest token, 103 with five, 113 with twenty) and 176 us backward (94 %); 4096
-// rows of 32003 fp32 83 us (97 %; 90 us with the likeliest). Long rows are bound by memory, bf16
+// Measured (one B200, copy rate 6.54 TB/s, L2 cold): 8192 rows of 32768 bf16 90 to 92 us forward (91 to 89 % of the copy
+// rate; 104 us with the likeliest token, 107 with five, 116 with twenty) and 175 us backward (94 %); 4096
+// rows of 32003 fp32 83 to 88 us (97 to 91 %; 90 to 95 us with the likeliest). Long rows are bound by memory, bf16
 // ones nearly as much by instructions (issue slots 80 % used: an element costs an exponential, a
 // difference, a product, two sums and a maximum); short rows by what each row's end costs (20000 rows of
-// 4096 bf16 41 us, 61 %), a few rows by latency (33 rows of 32768 bf16 with five alternatives 6.2 us).
+// 4096 bf16 41 us, 61 %), a few rows by latency (33 rows of 32768 bf16 with five alternatives 6.3 us). Some hundreds of long
+// rows leave SMs short of loads (300 rows of 32768 bf16 11.5 us for 3 us of bytes, 600 13), and a gradient of few long
+// rows has one CTA a row (33 rows of 150000 fp32 57 us for 6).
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/types.h>

@@ -4,7 +4,7 @@
 
 namespace hrm {
 
-constexpr int kUnitKeys = 128;  // keys of one unit: 16 for each of a CTA's 8 warps
+constexpr int kUnitKeys = 128;  // keys of one unit: 32 for each of a CTA's 4 warps
 // What starting and finishing a (request, head) costs, in units: first loads, merging the warps, writing.
 constexpr int kPairCost = 3;
 

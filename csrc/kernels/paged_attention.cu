@@ -38,14 +38,16 @@
 // the first (of the scores, for the sum of P). So each product keeps its 11 bits whatever ranges the row's blocks have, and
 // one that is lost is below 2^-24 of the row's largest.
 //
-// Measured (one B200, copy rate 6.54 TB/s): 16 requests of 4000 to 40000 tokens, 8 kv heads, 4 query
-// heads each, int8: 100 us for 632 MB (97 % of the copy rate); 100 requests of 1 to 4096 tokens, 12 heads,
-// e4m3: 104 us for 663 MB (98 %). Small calls are bound by dependent loads and launches: one
-// request of 777 tokens 6.8 us, 33 requests around 600 tokens 17 us for 46 MB, of which about 5 us
-// pass before the first codes arrive. With 8 to 16 rows (12 requests of 300 to 6000 tokens, up to 7 new
-// ones, 2 query heads) 26 us for 96 MB: the latency of a step's chains (11 warps an SM, 46 % of the issue
-// slots used). 3 CTAs an SM (168 registers) hold 12 warps with 8 KB each in flight; 2 CTAs of 8 warps
-// with 4 KB steps were 6 and 18 % slower on the first two cases.
+// Measured (one B200, copy rate 6.54 TB/s, L2 cold): 16 requests of 4000 to 40000 tokens, 8 kv heads, 4 query
+// heads each, int8: 98 us for 632 MB (99 % of the copy rate); 100 requests of 1 to 4096 tokens, 12 heads,
+// e4m3: 102 us for 663 MB (99 %). Small calls are bound by dependent loads and launches: one
+// request of 777 tokens 6.3 us, 33 requests around 600 tokens 16 us (e4m3: 15) for 46 MB, of which about 5 us
+// pass before the first codes arrive; the join ends some 2 us later. With 8 to 16 rows (12 requests of 300 to 6000
+// tokens, up to 7 new ones, 2 query heads) 26 us (int8: 27) for 96 MB: the latency of a step's chains (11 warps an SM,
+// 49 % of the issue slots used). Many new tokens read and widen the codes again for each 16 rows: 2048 on 2048
+// cached, 10 heads, 214 us (e4m3: 196), of which the products at the bf16 rate would be 26. 3 CTAs an SM (168
+// registers) hold 12 warps with 8 KB each in flight; 2 CTAs of 8 warps with 4 KB steps were 6 and 18 % slower on the
+// first two cases.
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <cuda_fp16.h>

@@ -22,7 +22,7 @@
 // (a counter that it puts back to zero) moves lengths and num_free, after every CTA has read
 // them. These calls are bound by launch and dependent-load latency, not by bytes: a truncate and a
 // decode step of 25 requests take 8 us together, a truncate and the step of 512 prompts of half a million tokens
-// 12 us (15 us with one row a thread; 8 CTAs an SM instead of 2 were 2.5 us slower, the prefix sums again in
+// 11 us (15 us with one row a thread; 8 CTAs an SM instead of 2 were 2.5 us slower, the prefix sums again in
 // each).
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>

@@ -4,14 +4,15 @@ A paged cache stores the keys and values of one attention layer in blocks of ``b
 tokens, as int8 or e4m3 codes with one fp32 scale for each block and head. Requests own blocks
 through ``BlockTables``, which all layers of a model share. One step of generation is
 
-    plan = tables.step(new_tokens, num_tokens)            # once: blocks, slots, positions
+    plan = tables.step(new_tokens, num_tokens, max_new=1) # once: blocks, slots, positions
     for every layer:
         paged_append(key, value, cache, plan)             # [num_tokens, heads, 128] bf16
         y = paged_attention(query, cache, plan, gate=gate)
     tables.truncate(keep)                                 # a request that ends frees its blocks
 
 Nothing here reads a device value on the host, so a step can be captured in a CUDA graph and
-replayed. Everything runs on the current stream; a plan, its tables and the caches are used in stream order.
+replayed. Everything runs on the current stream; a plan, its tables and the caches are used in stream order. These
+calls are for inference: their results carry no gradient.
 On CUDA the kernels of csrc/kernels/paged_*.cu run. ``BlockTables`` on the CPU, and
 ``models.paged`` for the rest, are the plain torch oracle of the same operations.
 
@@ -144,7 +145,7 @@ class BlockTables:
         """Give every request room for ``new_tokens [R]`` more tokens (int32, on the tables' device).
 
         ``num_tokens`` is the number of packed rows of the step, at least the sum of ``new_tokens``;
-        ``max_new`` bounds one request's (a decode step: 1). A step that does not fit does nothing: its plan is
+        ``max_new`` bounds one request's (a decode step: 1; attention takes a kernel for few rows where it is small). A step that does not fit does nothing: its plan is
         empty, and ``check`` raises.
         """
         self._check(new_tokens, "new_tokens")
@@ -158,7 +159,8 @@ class BlockTables:
         return step_reference(self, new_tokens, num_tokens, max_new)
 
     def truncate(self, keep: Tensor) -> None:
-        """Cut every request to at most ``keep [R]`` tokens (int32) and free its surplus blocks."""
+        """Cut every request to at most ``keep [R]`` tokens (int32) and free its surplus blocks. A block that stays in
+        part keeps its codes and scales, a scale that tokens now cut had widened among them."""
         self._check(keep, "keep")
         if self.tables.is_cuda:
             cuda().paged_truncate(*self._state, keep)
