@@ -70,6 +70,7 @@ constexpr int kHalf = 2 * 16 * D;          // bytes of 16 keys: codes of keys, t
 constexpr int kStage = 2 * kHalf;
 constexpr int kStages = 2;      // one is read while the other is filled
 constexpr int kPart = D + 4;    // floats of a row's part, in whole 16 bytes
+constexpr int kFewTiles = 4;    // up to these the grid has each nominal tile's workers
 constexpr float kLazy = 8.f;    // a running maximum may lag by 2^8: P stays below 256 in f16
 constexpr float kNoUnit = 1e30f;  // in place of log2(2^m / O's unit) before a value was met: O is 0
 constexpr float kMostRatio = 126.f;  // where 2^m / unit * scale is larger, P is 0
@@ -124,7 +125,7 @@ __device__ __forceinline__ Place place_of(const AttnArgs& a, const Found& mine) 
     __syncthreads();
     for (int w = 0; w < (int)blockDim.x / 32; ++w) n = max(n, s_most[w]);
     const int tiles = max(1, (int)(((long)n * a.G + ROWS - 1) / ROWS));
-    p.workers = max(1, a.split / tiles);
+    p.workers = max(1, a.split / max(tiles, kFewTiles));  // few: as with a grid that says so
     p.worker = blockIdx.x % p.workers;
     p.tile = blockIdx.x / p.workers;
     p.none = p.tile >= tiles;
@@ -776,11 +777,11 @@ void launch(AttnArgs a, int max_rows, const at::TensorOptions& opts) {
   constexpr int ROWS = 8 * NT, smem = kWarps * kStages * kStage;
   const int tiles = (max_rows + ROWS - 1) / ROWS;
   C10_CUDA_CHECK(ensure_dynamic_smem((const void*)paged_attention_kernel<FP8, NT>, smem));
-  // up to four tiles: each is cut among as many CTAs as fit the SMs. More (a request with many new tokens, or a step
+  // up to kFewTiles tiles: each is cut among as many CTAs as fit the SMs. More (a request with many new tokens, or a step
   // that does not say how many one may have): four waves of CTAs among the tiles that the step turns out to have, at
   // least one a tile. The workspace is under 32 MB either way.
   const int resident = device_sm_count() * 3;
-  a.split = tiles <= 4 ? 0 : 4 * resident;
+  a.split = tiles <= kFewTiles ? 0 : kFewTiles * resident;
   const at::Tensor part = at::empty({2L * (a.split ? a.split : resident * tiles) * ROWS * kPart}, opts.dtype(at::kFloat));
   a.part = part.data_ptr<float>();
   const dim3 grid = a.split ? dim3(std::max(a.split, tiles)) : dim3(resident, tiles);

@@ -308,3 +308,25 @@ def test_late_tiles_see_exactly_their_keys(cuda_device, dtype, chunk, group, siz
     want = paged_attention_reference(q.double(), cache, plan, dtype=torch.float64)
     top = float(cache.value_scales.max()) * (127 if dtype == torch.int8 else 448)
     assert ((out.double() - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -10 * top).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("most", [5, 17, 32])
+def test_few_rows_with_a_loose_bound(cuda_device, dtype, most):
+    """One to four tiles of rows a request, nominally many: cut as with the tight bound, to the same bits."""
+    from hrm_text_b200.ops.paged import BlockTables, PagedKV8, paged_append, paged_attention
+    torch.manual_seed(most)
+    new = [1 + (i * 5) % most for i in range(80)]
+    old = [(i * 37) % 900 for i in range(80)]
+    bt = BlockTables(80 * 30, 32, 80, 30, cuda_device)
+    cache = PagedKV8.create(80 * 30, 32, 3, dtype, cuda_device)
+    for step in (old, new):
+        rows = sum(step)
+        plan = bt.step(_i32(step, cuda_device), rows)
+        x = torch.randn(rows, 2, 3, 128, device=cuda_device).bfloat16()
+        paged_append(x[:, 0], x[:, 1], cache, plan)
+    bt.check()
+    q = torch.randn(rows, 6, 128, device=cuda_device).bfloat16()
+    out = paged_attention(q, cache, plan)
+    _bound(out, q, cache, plan)
+    assert torch.equal(out, paged_attention(q, cache, plan._replace(max_new=max(new))))
